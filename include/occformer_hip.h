@@ -623,6 +623,52 @@ int occf_image_crop_rotate_normalize_fwd(const uint8_t* in, float* out, uint8_t*
                                          int fW, int fH, int flip, int rot_mode, const int64_t* affine, const float* mean,
                                          const float* stdinv, int to_rgb, void* stream);
 
+/* ------------------------------------------------------------------ position operators - */
+/* dtype of these entry points: 0 = fp32, 1 = bf16 (q, k, v, weights, tables and their gradients alike); sums, statistics and
+ * workspaces are fp32. */
+
+/* Norms of queries and keys for each head and the position rotation, one pass over both.  A row is one head of a token:
+ * y = x / sqrt(mean(x^2) + eps) * weight; of y's first 2 * half columns the pairs (c, c + half) -- interleaved: (2c, 2c + 1)
+ * -- are turned by the angle whose cosine / sine is row `position`, column c of cos / sin[table rows, half]; the others pass.
+ * With several position axes column c belongs to axis 0 below cut1, 1 below cut2, else 2.  positions NULL: the token's index.
+ * A position outside the table makes the turned columns of its rows NaN.
+ * geom = { B, L, Hq, Hk (0: no keys), D (even, <= 128), 2 * half, table rows, axes (1..3), cut1, cut2,
+ *          positions a batch entry (0: shared by the batch), q strides of batch / token / head, k strides } (elements; the
+ * head's columns are contiguous).  q_out [B, L, Hq, D], k_out [B, L, Hk, D] contiguous, 16-byte aligned. */
+int occf_qk_norm_rope_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                          const float* sin, const int32_t* positions, void* q_out, void* k_out, const int64_t* geom,
+                          float eps, int interleaved, int dtype, void* stream);
+
+/* Its backward: dq_out / dk_out, dq / dk contiguous; q_weight / k_weight gradients [D] summed in a fixed order.
+ * workspace: occf_qk_norm_rope_bwd_workspace(D) floats. */
+long occf_qk_norm_rope_bwd_workspace(int head_dim);
+int occf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* cos,
+                          const float* sin, const int32_t* positions, const void* dq_out, const void* dk_out, void* dq,
+                          void* dk, void* dq_weight, void* dk_weight, float* workspace, const int64_t* geom, float eps,
+                          int interleaved, int dtype, void* stream);
+
+/* Attention with a learned relative position bias by buckets: t = scale q.k + table[lut[clamp(j - p_i, -R, R) + R], head],
+ * p_i = q_start[b] + i; softmax over the keys j < k_lens[b] (causal: j <= p_i); rows i >= q_lens[b] and rows without a key are
+ * zeros.  q_lens / k_lens / q_start NULL: all rows, all keys, 0.  A table entry at or below -1e30 takes its bucket out.
+ * geom = { B, Lq, Lk, Hq, Hk (divides Hq: query head h reads key head h / (Hq / Hk)), D (multiple of 8, <= 128),
+ *          buckets (<= 128), R (<= 1024), q strides of batch / row / head, k strides, v strides } (elements, 16-byte
+ * multiples; pointers 16-byte aligned).  table [buckets, Hq], lut [2 R + 1], out [B, Lq, Hq, D] contiguous,
+ * lse [B, Hq, Lq] (may be NULL) = base-2 logarithm of a row's sum of exponentials (-inf: no key), what the backward reads.
+ * workspace: occf_rel_attn_workspace floats (0: may be NULL; negative: arguments outside the limits). */
+long occf_rel_attn_workspace(const int64_t* geom, int dtype);
+int occf_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
+                      const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_start, void* out, float* lse,
+                      float* workspace, long workspace_floats, const int64_t* geom, float scale, int causal, int dtype,
+                      void* stream);
+
+/* Its backward: out / lse as the forward left them, dout [B, Lq, Hq, D]; dq [B, Lq, Hq, D], dk / dv [B, Lk, Hk, D] (rows that
+ * do not count are zeros), dtable [buckets, Hq].  Every sum in a fixed order: two runs give the same bits. */
+long occf_rel_attn_bwd_workspace(const int64_t* geom, int dtype);
+int occf_rel_attn_bwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
+                      const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_start, const void* out,
+                      const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable, float* workspace,
+                      long workspace_floats, const int64_t* geom, float scale, int causal, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

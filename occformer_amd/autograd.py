@@ -1,5 +1,5 @@
 """torch.autograd.Function wrappers that pair every forward entry point of liboccformer_hip.so with its hand-written
-backward (csrc/bwd_elem.hip, wgrad.hip, attn_bwd.hip, msda3d.hip, dcn.hip, lss.hip) -- the training step of the path.
+backward (csrc/bwd_elem.hip, wgrad.hip, attn_bwd.hip, msda3d.hip, dcn.hip, lss.hip, qk_norm_rope.hip, rel_attn_bwd.hip) -- the training step of the path.
 
 The reference's counterpart is ATen autograd through the PyTorch modules plus ``QuickCumsumCuda``
 (mmdet3d/ops/bev_pool/bev_pool.py:37-80); ``loss.backward()`` of ``OccupancyFormer.forward_train``
@@ -593,6 +593,55 @@ class MaskedAttention(torch.autograd.Function):
         q, k, v, out = ctx.saved_tensors
         dq, dk, dv = get_ops().masked_attention_backward(q, k, v, ctx.heads, out, dout.contiguous(), *ctx.mask)
         return dq, dk, dv, None, None, None
+
+
+class QkNormRope(torch.autograd.Function):
+    """``ops.qk_norm_rope`` with its backward; no gradient for the tables and positions"""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, axis_dims, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.cfg = (eps, axis_dims, interleaved)
+        return get_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, axis_dims, interleaved)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        dq_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if dq_out is None else dq_out
+        if k is not None and dk_out is None:
+            dk_out = torch.zeros(k.shape, dtype=k.dtype, device=k.device)
+        dq, dk, dqw, dkw = get_ops().qk_norm_rope_backward(q, k, q_weight, k_weight, dq_out, dk_out, cos, sin, positions,
+                                                           *ctx.cfg)
+        return dq, dk, dqw, dkw, None, None, None, None, None, None
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos=None, sin=None, positions=None, eps=1e-6, axis_dims=None, interleaved=False):
+    """``ops.qk_norm_rope`` in the training graph"""
+    return QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, axis_dims, interleaved)
+
+
+class RelAttention(torch.autograd.Function):
+    """``ops.rel_attention`` with its backward (q, k, v and the bias table)"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, scale, causal, q_lens, k_lens, q_start):
+        out, lse = get_ops().rel_attention(q, k, v, table, buckets, scale, causal, q_lens, k_lens, q_start, return_lse=True)
+        ctx.save_for_backward(q, k, v, table, out, lse, q_lens, k_lens, q_start)
+        ctx.cfg = (buckets, scale, causal)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, table, out, lse, q_lens, k_lens, q_start = ctx.saved_tensors
+        buckets, scale, causal = ctx.cfg
+        dq, dk, dv, dtable = get_ops().rel_attention_backward(q, k, v, table, buckets, out, lse, dout, scale, causal, q_lens,
+                                                              k_lens, q_start)
+        return dq, dk, dv, dtable, None, None, None, None, None, None
+
+
+def rel_attention(q, k, v, table, buckets, scale=None, causal=False, q_lens=None, k_lens=None, q_start=None):
+    """``ops.rel_attention`` in the training graph"""
+    return RelAttention.apply(q, k, v, table, buckets, scale, causal, q_lens, k_lens, q_start)
 
 
 class PointSample3d(torch.autograd.Function):

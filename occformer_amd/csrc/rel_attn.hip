@@ -1,0 +1,494 @@
+// Attention with a learned relative position bias by buckets: forward.
+//
+//   t_ij = scale q_i.k_j + T[bucket(j - p_i), h],  p_i = q_start + i;   o_i = sum_j softmax_j(t_ij) v_j
+//
+// over the pairs that count (j < k_len, i < q_len, and j <= p_i when causal).  The reference has a learned position bias in
+// its window attention only (projects/mmdet3d_plugin/occformer/backbones/modules/window_attention.py:69-107: a table over the
+// 169 offsets of a 7 x 7 window); here the distance is any length and the table has one row a bucket of distances.
+//
+// Neither the scores nor the bias exist in memory.  The bucket function is a table over the clamped distance (-R .. R), so a
+// head's bias is 2 R + 1 floats in LDS: a 32 x 32 score tile wholly further than R from the diagonal adds a constant (folded
+// into the exponent's fma), any other reads its 16 values a lane at constant offsets from one address.
+#include "rel_attn.h"
+#include "../../include/occformer_hip.h"
+
+#define RA_EXCEED 8.0f          // the running maximum follows only when a tile exceeds it by 2^8: p <= 256, sums stay fp32
+
+// one 32-key score tile of a lane: t (base 2, biased, masked) from the raw products s; returns its maximum
+// jl = j0 + 4 lk; pi = position of this lane's query
+template <bool MASK>
+__device__ __forceinline__ float ra_scores(f32x16& s, const float* lut, const RaParams& p, int j0, int pi, int lk, int nk,
+                                           bool near, float far) {
+  float mx = -INFINITY;
+  const int jl = j0 + 4 * lk;
+  const float* bl = lut + (near ? jl - pi + p.R + RA_PAD : 0);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int o = (r & 3) + 8 * (r >> 2);
+    float t = near ? fmaf(s[r], p.c, bl[o]) : fmaf(s[r], p.c, far);
+    if (MASK) {
+      const int j = jl + o;
+      if (j >= nk || (p.causal && j > pi)) t = -INFINITY;
+    }
+    s[r] = t;
+    mx = fmaxf(mx, t);
+  }
+  return mx;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Many queries: a workgroup owns 128 queries of one head, a wave 32 of them (a lane one query: its running maximum and sum
+// are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.
+template <class T, int DP, int KT>
+__global__ void __launch_bounds__(256) rel_attn_fwd_kernel(RaParams p) {
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
+  constexpr int NB = KT * DP / 16, NU = (NB + 255) / 256;               // 4 x 4 blocks of a tile, and a thread's share
+  OCCF_DYN_SMEM(smem);
+  char* img_k = smem;
+  char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
+  float* lut = (float*)(img_v + NT * RaTrans<KT>::bytes(DP));
+
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  const int nqt = (p.Lq + 127) / 128;
+  unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
+  const int qt = nqt - 1 - (int)(bid % nqt);            // causal: the longest rows first
+  bid /= nqt;
+  const int h = (int)(bid % p.Hq), b = (int)(bid / p.Hq);
+  const int hk = h / (p.Hq / p.Hk);
+  int nq, nk, start;
+  ra_lengths(p, b, nq, nk, start);
+
+  ra_fill_bias<T>(lut, p, h, tid, 256);
+
+  const int i0 = qt * 128 + wave * 32, i = i0 + li;
+  const int pi = start + i;
+  const T* qrow = (const T*)p.q + (long)b * p.qsb + (long)occf_clampi(i, p.Lq - 1) * p.qsl + (long)h * p.qsh;
+  RaFrag<NT> qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int d = ks * 16 + lk * 8;
+    qf[ks] = ra_row_frag<T>(qrow + (d < p.D ? d : 0), i < nq && d < p.D);
+  }
+
+  // keys of this workgroup: all, or up to its last query's position
+  int kend = nk;
+  if (p.causal) {
+    const int last = start + (qt * 128 + 128 < nq ? qt * 128 + 128 : nq);      // behind the last query
+    kend = last < kend ? (last > 0 ? last : 0) : kend;
+  }
+  if (qt * 128 >= nq) kend = 0;
+  const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
+  const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+
+  RaBlk<T> rk[NU], rv[NU];
+  const int ntile = (kend + KT - 1) / KT;
+  if (ntile > 0) {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      if (NB % 256 && tid + n * 256 >= NB) break;
+      ra_load_blk<T, DP>(rk[n], kb, p.ksl, 0, kend, p.D, tid + n * 256);
+      ra_load_blk<T, DP>(rv[n], vb, p.vsl, 0, kend, p.D, tid + n * 256);
+    }
+  }
+  for (int kt = 0; kt < ntile; ++kt) {
+    const int k0 = kt * KT;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      if (NB % 256 && tid + n * 256 >= NB) break;
+      uint32_t w[NT][4][2];
+      ra_blk_pieces(rk[n], w);
+      ra_store_row<NT, DP, KT>(img_k, w, tid + n * 256);
+      ra_blk_pieces(rv[n], w);
+      ra_store_trans<NT, DP, KT>(img_v, w, tid + n * 256);
+    }
+    __syncthreads();
+    if (kt + 1 < ntile) {
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        if (NB % 256 && tid + n * 256 >= NB) break;
+        ra_load_blk<T, DP>(rk[n], kb, p.ksl, k0 + KT, kend, p.D, tid + n * 256);
+        ra_load_blk<T, DP>(rv[n], vb, p.vsl, k0 + KT, kend, p.D, tid + n * 256);
+      }
+    }
+    if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
+    f32x16 s[KT / 32];
+#pragma unroll
+    for (int sub = 0; sub < KT / 32; ++sub) {
+      s[sub] = ra_zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s[sub] = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s[sub]);
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int sub = 0; sub < KT / 32; ++sub) {
+      const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);           // tile distances: rel0 - 31 .. rel0 + 31
+      const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
+      const float far = lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD];
+      const bool mask = j0 + 32 > kend || (p.causal && j0 + 31 > start + i0);
+      const float x = mask ? ra_scores<true>(s[sub], lut, p, j0, pi, lk, kend, near, far)
+                           : ra_scores<false>(s[sub], lut, p, j0, pi, lk, kend, near, far);
+      mx = fmaxf(mx, x);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__ballot(mx > m + RA_EXCEED)) {
+      const float mn = fmaxf(m, mx);
+      const float a = ra_exp2(m - (mn == -INFINITY ? 0.f : mn));       // first keys of a row: exp2(-inf) = 0
+      m = mn;
+      mref = mn == -INFINITY ? 0.f : mn;
+      l *= a;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
+    }
+#pragma unroll
+    for (int sub = 0; sub < KT / 32; ++sub) {
+      float pv[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        pv[r] = ra_exp2(s[sub][r] - mref);
+        l += pv[r];
+      }
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, KT>(img_v, dt * 32, sub * 2 + s2, li, lk), pf, acc[dt]);
+      }
+    }
+  }
+  if (i >= p.Lq) return;
+  l += __shfl_xor(l, 32);
+  const bool some = l > 0.f && i < nq;                   // rows behind the last query went along with their tile
+  const float inv = some ? 1.0f / l : 0.f;
+  if (!some) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+  }
+  T* orow = (T*)p.o + (((long)b * p.Lq + i) * p.Hq + h) * p.D;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = dt * 32 + 8 * g + 4 * lk;
+      if (d < p.D)
+        ra_store4(orow + d, acc[dt][4 * g] * inv, acc[dt][4 * g + 1] * inv, acc[dt][4 * g + 2] * inv, acc[dt][4 * g + 3] * inv);
+    }
+  if (p.lse && lk == 0) p.lse[((long)b * p.Hq + h) * p.Lq + i] = some ? m + ra_log2(l) : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Few queries: the rows of one key head (query i of its G query heads, row = i G + g) in groups of 32 share every key that
+// is read.  The keys are split over workgroups and, tile by tile, over a workgroup's four waves; a wave reads its
+// key rows straight into operand registers and turns its value rows round in LDS of its own, so that no wave waits for
+// another before the join at the end.  part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
+template <class T, int DP>
+struct RaFew {
+  static constexpr int NT = RaType<T>::NT, VT = NT * RaTrans<32>::bytes(DP);
+  static constexpr int join = 32 * (DP + 4) * 4;         // [32 rows][DP + 4] floats of one wave
+  static constexpr int wave = VT > join ? VT : join;
+};
+
+template <class T, int DP>
+__global__ void __launch_bounds__(256) rel_attn_few_kernel(RaParams p) {
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
+  constexpr int NB = 2 * DP, NV = (NB + 63) / 64;                        // 4 x 4 blocks of 32 value rows, and a lane's share
+  OCCF_DYN_SMEM(smem);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  char* img_v = smem + wave * RaFew<T, DP>::wave;
+  float* tab = (float*)(smem + RA_WAVES * RaFew<T, DP>::wave);          // [nb][32] bias of row li
+  int* lut = (int*)(tab + p.nb * 32);                                   // [2 R + 1] bucket of a distance
+  float* stat = (float*)(lut + 2 * p.R + 1);                            // [2 RA_WAVES + 2][32]
+
+  const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
+  const unsigned split = blockIdx.x % p.nsplit, group = blockIdx.x / p.nsplit;
+  unsigned bid = group;
+  const int rt = (int)(bid % nrt);
+  bid /= nrt;
+  const int hk = (int)(bid % p.Hk), b = (int)(bid / p.Hk);
+  int nq, nk, start;
+  ra_lengths(p, b, nq, nk, start);
+  const int row = rt * 32 + li;
+  const int i = row / G, h = hk * G + row % G;
+  const bool live = row < rows && i < nq;
+  const int pi = start + i;
+  const int i_first = (rt * 32) / G, i_last = (rt * 32 + 31 < rows ? rt * 32 + 31 : rows - 1) / G;
+
+  for (int t = tid; t < p.nb * 32; t += 256) {
+    const int r = rt * 32 + (t & 31);
+    tab[t] = r < rows ? ra_bias(ra_to_float(((const T*)p.table)[(long)(t >> 5) * p.Hq + hk * G + r % G])) : 0.f;
+  }
+  for (int t = tid; t < 2 * p.R + 1; t += 256) lut[t] = occf_clampi(p.lut[t], p.nb - 1) * 32;
+
+  const T* qrow = (const T*)p.q + (long)b * p.qsb + (long)(live ? i : 0) * p.qsl + (long)(live ? h : 0) * p.qsh;
+  RaFrag<NT> qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int d = ks * 16 + lk * 8;
+    qf[ks] = ra_row_frag<T>(qrow + (d < p.D ? d : 0), live && d < p.D);
+  }
+  int kend = nk;
+  if (p.causal) {
+    const int last = start + (i_last < nq ? i_last : nq - 1) + 1;
+    kend = last < kend ? (last > 0 ? last : 0) : kend;
+  }
+  if (i_first >= nq) kend = 0;
+  const int first = split * p.chunk;
+  const int lim = first + p.chunk < kend ? first + p.chunk : kend;
+  const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
+  const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
+  __syncthreads();
+
+  f32x16 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+
+  RaFrag<NT> kf[KS];
+  RaBlk<T> rv[NV];
+  int j0 = first + wave * 32;
+  auto load = [&](int at) {
+    const bool ok = at + li < lim;
+    const T* krow = kb + (long)(ok ? at + li : 0) * p.ksl;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + lk * 8;
+      kf[ks] = ra_row_frag<T>(krow + (d < p.D ? d : 0), ok && d < p.D);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T, DP>(rv[n], vb, p.vsl, at, lim, p.D, lane + n * 64);
+  };
+  if (j0 < lim) load(j0);
+  for (; j0 < lim; j0 += RA_WAVES * 32) {
+    f32x16 s = ra_zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = ra_mm<NT>(kf[ks], qf[ks], s);
+    RA_WAVE_SYNC();
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+      if (NB % 64 == 0 || lane + n * 64 < NB) {
+        uint32_t w[NT][4][2];
+        ra_blk_pieces(rv[n], w);
+        ra_store_trans<NT, DP, 32>(img_v, w, lane + n * 64);
+      }
+    RA_WAVE_SYNC();
+    if (j0 + RA_WAVES * 32 < lim) load(j0 + RA_WAVES * 32);
+
+    const int lo = j0 - (start + i_last), hi = j0 + 31 - (start + i_first);        // distances of the tile
+    float mx = -INFINITY;
+    if (hi <= -p.R || lo >= p.R) {
+      const float far = tab[lut[hi <= -p.R ? 0 : 2 * p.R] + li];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.c, far);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int rel = j0 + 4 * lk + (r & 3) + 8 * (r >> 2) - pi;
+        s[r] = fmaf(s[r], p.c, tab[lut[occf_clampi(rel + p.R, 2 * p.R)] + li]);
+      }
+    }
+    if (j0 + 32 > lim || (p.causal && j0 + 31 > start + i_first)) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = j0 + 4 * lk + (r & 3) + 8 * (r >> 2);
+        if (j >= lim || (p.causal && j > pi)) s[r] = -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__ballot(mx > m + RA_EXCEED)) {
+      const float mn = fmaxf(m, mx);
+      const float a = ra_exp2(m - (mn == -INFINITY ? 0.f : mn));
+      m = mn;
+      mref = mn == -INFINITY ? 0.f : mn;
+      l *= a;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
+    }
+    float pv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      pv[r] = ra_exp2(s[r] - mref);
+      l += pv[r];
+    }
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, li, lk), pf, acc[dt]);
+    }
+  }
+  l += __shfl_xor(l, 32);
+  if (!live) {                                           // rows behind the last query went along with their tile
+    l = 0.f;
+    m = -INFINITY;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+  }
+
+  // ---- join the four waves: maxima and sums first, then the rescaled accumulators in wave order
+  if (lk == 0) {
+    stat[wave * 32 + li] = m;
+    stat[(RA_WAVES + wave) * 32 + li] = l;
+  }
+  __syncthreads();
+  float mj = -INFINITY, lj = 0.f;
+#pragma unroll
+  for (int w = 0; w < RA_WAVES; ++w) mj = fmaxf(mj, stat[w * 32 + li]);
+  const float mz = mj == -INFINITY ? 0.f : mj;
+#pragma unroll
+  for (int w = 0; w < RA_WAVES; ++w) lj += stat[(RA_WAVES + w) * 32 + li] * ra_exp2(stat[w * 32 + li] - mz);
+  const float a = ra_exp2(m - mz);
+  float* jo = (float*)img_v;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      ra_store4(jo + li * (DP + 4) + dt * 32 + 8 * g + 4 * lk, acc[dt][4 * g] * a, acc[dt][4 * g + 1] * a,
+                acc[dt][4 * g + 2] * a, acc[dt][4 * g + 3] * a);
+  float* joined = stat + 2 * RA_WAVES * 32;
+  if (wave == 0 && lk == 0) {
+    joined[li] = mj;
+    joined[32 + li] = lj;
+  }
+  __syncthreads();
+  for (int u = tid; u < 32 * (DP / 4); u += 256) {
+    const int r = u / (DP / 4), d = (u % (DP / 4)) * 4;
+    const int rw = rt * 32 + r;
+    if (rw >= rows || d >= p.D) continue;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < RA_WAVES; ++w) {
+      const float4 y = *(const float4*)((float*)(smem + w * RaFew<T, DP>::wave) + r * (DP + 4) + d);
+      x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
+    }
+    const float lr = joined[32 + r], mr = joined[r];
+    const int ri = rw / G, rh = hk * G + rw % G;
+    if (p.part) {
+      float* ph = p.part + ((long)split * (gridDim.x / p.nsplit) + group) * (32 * (p.D + 2));
+      ra_store4(ph + 64 + r * p.D + d, x[0], x[1], x[2], x[3]);
+      if (d == 0) {
+        ph[r] = mr;
+        ph[32 + r] = lr;
+      }
+    } else {
+      const float inv = lr > 0.f ? 1.0f / lr : 0.f;
+      ra_store4((T*)p.o + (((long)b * p.Lq + ri) * p.Hq + rh) * p.D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+      if (p.lse && d == 0) p.lse[((long)b * p.Hq + rh) * p.Lq + ri] = lr > 0.f ? mr + ra_log2(lr) : -INFINITY;
+    }
+  }
+}
+
+// joins the splits of rel_attn_few_kernel in their order: one thread four columns of a row
+template <class T>
+__global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p, int groups) {
+  const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
+  const int dq = p.D / 4;
+  const long u = (long)blockIdx.x * 256 + threadIdx.x;
+  const int d = (int)(u % dq) * 4;
+  const long rw_all = u / dq;
+  if (rw_all >= (long)p.B * p.Hk * rows) return;
+  const int rw = (int)(rw_all % rows);
+  const long bh = rw_all / rows;
+  const int hk = (int)(bh % p.Hk), b = (int)(bh / p.Hk);
+  const int r = rw & 31;
+  const float* ph = p.part + (bh * nrt + (rw >> 5)) * (32 * (p.D + 2));
+  const long step = (long)groups * (32 * (p.D + 2));
+  float m = -INFINITY;
+  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, ph[s * step + r]);
+  const float mz = m == -INFINITY ? 0.f : m;
+  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.nsplit; ++s) {
+    const float a = ra_exp2(ph[s * step + r] - mz);
+    l = fmaf(ph[s * step + 32 + r], a, l);
+    const float4 y = *(const float4*)(ph + s * step + 64 + r * p.D + d);
+    x[0] = fmaf(y.x, a, x[0]);
+    x[1] = fmaf(y.y, a, x[1]);
+    x[2] = fmaf(y.z, a, x[2]);
+    x[3] = fmaf(y.w, a, x[3]);
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const int i = rw / G, h = hk * G + rw % G;
+  ra_store4((T*)p.o + (((long)b * p.Lq + i) * p.Hq + h) * p.D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+  if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.Lq + i] = l > 0.f ? m + ra_log2(l) : -INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// How a call is run.  The few-query kernel wins while the workgroups of the other one would not fill the card.
+static void ra_plan(const int64_t* g, int& few, int& nsplit, int& chunk) {
+  const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
+  const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32);
+  few = rows <= 32 || B * Hq * ((Lq + 127) / 128) < 128;
+  nsplit = 1;
+  long c = Lk;
+  if (few) {
+    // about two workgroups a compute unit, none with less than 128 keys (a 32-key tile a wave)
+    long want = (512 + groups - 1) / groups;
+    const long most = (Lk + 127) / 128;
+    want = want < 1 ? 1 : (want > most ? (most < 1 ? 1 : most) : want);
+    want = want > 64 ? 64 : want;
+    c = (Lk + want - 1) / want;
+    c = (c + 127) / 128 * 128;
+    nsplit = (int)((Lk + c - 1) / c);
+    if (nsplit < 1) nsplit = 1;
+  }
+  chunk = (int)c;
+}
+
+template <class T, int DP>
+static int ra_fwd(RaParams& p, int few, void* stream) {
+  if (few) {
+    const int rows = p.Lq * (p.Hq / p.Hk), groups = p.B * p.Hk * ((rows + 31) / 32);
+    const size_t lds = RA_WAVES * RaFew<T, DP>::wave + 4 * ((size_t)p.nb * 32 + 2 * p.R + 1 + (2 * RA_WAVES + 2) * 32);
+    int rc = ra_launch(rel_attn_few_kernel<T, DP>, dim3((unsigned)((long)p.nsplit * groups)), 256, lds, stream, p);
+    if (rc || !p.part) return rc;
+    const long n = (long)p.B * p.Hk * rows * (p.D / 4);
+    hipLaunchKernelGGL(rel_attn_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p, groups);
+    OCCF_LAUNCH_CHECK();
+  }
+  constexpr int NT = RaType<T>::NT, KT = NT == 3 && DP > 64 ? 32 : 64;
+  const size_t lds = NT * (RaRow<DP>::bytes(KT) + RaTrans<KT>::bytes(DP)) + 4 * (2 * (size_t)p.R + 1 + 2 * RA_PAD);
+  return ra_launch(rel_attn_fwd_kernel<T, DP, KT>, dim3((unsigned)((long)p.B * p.Hq * ((p.Lq + 127) / 128))), 256, lds,
+                   stream, p);
+}
+
+extern "C" long occf_rel_attn_workspace(const int64_t* geom, int dtype) {
+  if (ra_check(geom, dtype)) return -1;
+  int few, nsplit, chunk;
+  ra_plan(geom, few, nsplit, chunk);
+  if (!few || nsplit == 1) return 0;
+  const long rows = geom[1] * (geom[3] / geom[4]);
+  return (long)nsplit * geom[0] * geom[4] * ((rows + 31) / 32) * 32 * (geom[5] + 2);
+}
+
+extern "C" int occf_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
+                                 const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_start, void* out, float* lse,
+                                 float* workspace, long workspace_floats, const int64_t* geom, float scale, int causal,
+                                 int dtype, void* stream) {
+  const int bad = ra_check(geom, dtype);
+  if (bad) return bad;
+  if (!q || !k || !v || !table || !lut || !out || !(scale > 0.f)) return OCCF_EINVAL;
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) != 0) return OCCF_EINVAL;
+  int few;
+  RaParams p = ra_params(geom, scale, causal);
+  ra_plan(geom, few, p.nsplit, p.chunk);
+  const long need = occf_rel_attn_workspace(geom, dtype);
+  if (need > 0 && (!workspace || workspace_floats < need)) return OCCF_EINVAL;
+  p.q = q; p.k = k; p.v = v; p.table = table; p.lut = lut;
+  p.q_lens = q_lens; p.k_lens = k_lens; p.q_start = q_start;
+  p.o = out; p.lse = lse; p.part = need > 0 ? workspace : nullptr;
+  RA_DISPATCH(dtype, p.D, ra_fwd, p, few, stream);
+}

@@ -1188,6 +1188,217 @@ class HipOps:
                    deform_groups, self._stream())
         return dx, doff
 
+    # ------------------------------------------------------------------ position operators (csrc/qk_norm_rope.hip, rel_attn*.hip)
+    _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+    def _on_device(self, what, first, *others):
+        """all tensors of one call on one GPU (the library launches on that device's current stream) and of one type"""
+        for t in others:
+            if t is not None and t.device != first.device:
+                raise OccfError(f"{what}: tensors on {first.device} and {t.device}")
+        if self.strict and not first.is_cuda:
+            raise OccfError("occformer_amd ops need GPU tensors (no CPU path exists)")
+        if first.dtype not in self._DTYPES:
+            raise OccfError(f"{what}: fp32 or bf16 tensors expected, got {first.dtype}")
+        return self._DTYPES[first.dtype]
+
+    def _launch_on(self, t, name, *args):
+        """``_call`` with the stream of the tensors' own device, which need not be the current one"""
+        if t.is_cuda and t.device.index != torch.cuda.current_device():
+            with torch.cuda.device(t.device):
+                self._call(name, *args, self._stream())
+        else:
+            self._call(name, *args, self._stream())
+
+    @staticmethod
+    def _heads(what, name, t, dtype, heads=None, dim=None):
+        """[B, L, H, D] with contiguous columns, the other strides free (column blocks of a fused projection)"""
+        if t.dim() != 4 or t.dtype != dtype or t.numel() == 0:
+            raise OccfError(f"{what}: {name} must be a non-empty [B, L, H, D] tensor of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+        if (heads is not None and t.shape[2] != heads) or (dim is not None and t.shape[3] != dim):
+            raise OccfError(f"{what}: {name} {tuple(t.shape)} where {heads} heads of {dim} are expected")
+        return t if t.stride(3) == 1 else t.contiguous()
+
+    def _rotation(self, what, q, cos, sin, positions, axis_dims):
+        """-> (cos, sin, positions, columns turned, table rows, axes, cut1, cut2, positions a batch entry)"""
+        B, L, D = q.shape[0], q.shape[1], q.shape[3]
+        if cos is None and sin is None:
+            if positions is not None or axis_dims is not None:
+                raise OccfError(f"{what}: positions and axis_dims need the cos / sin table")
+            return None, None, None, 0, 0, 1, 0, 0, 0
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != self.f32 or \
+                sin.dtype != self.f32 or not 0 < 2 * cos.shape[1] <= D or cos.shape[0] < 1:
+            raise OccfError(f"{what}: cos and sin must be fp32 [positions, columns] tables with at most {D // 2} columns")
+        half = cos.shape[1]
+        dims = (half,) if axis_dims is None else tuple(int(n) for n in axis_dims)
+        if sum(dims) != half or not 1 <= len(dims) <= 3 or min(dims) < 1:
+            raise OccfError(f"{what}: axis_dims {dims} must be one to three counts that sum to the table's {half} columns")
+        A = len(dims)
+        per_b = 0
+        if positions is None:
+            if A > 1:
+                raise OccfError(f"{what}: several axes need positions [.., L, axes]")
+        else:
+            tail = (L,) if A == 1 and positions.dim() in (1, 2) and positions.shape[-1] == L else (L, A)
+            if positions.dtype != self.i32 or tuple(positions.shape) not in (tail, (B,) + tail, (1,) + tail):
+                raise OccfError(f"{what}: positions must be int32 {list(tail)} or {[B] + list(tail)}, got "
+                                f"{tuple(positions.shape)} of {positions.dtype}")
+            positions = positions.contiguous()
+            per_b = L * A if positions.numel() == B * L * A and B > 1 else 0
+        return cos.contiguous(), sin.contiguous(), positions, 2 * half, cos.shape[0], A, dims[0], \
+            (dims[0] + dims[1] if A > 1 else half), per_b
+
+    def _qk_norm_rope_args(self, what, q, k, q_weight, k_weight, cos, sin, positions, axis_dims, interleaved, grads=()):
+        dt = self._on_device(what, q, k, q_weight, k_weight, cos, sin, positions, *grads)
+        q = self._heads(what, "q", q, q.dtype)
+        B, L, Hq, D = q.shape
+        if D % 2 or D > 128:
+            raise OccfError(f"{what}: head dim {D} must be even and at most 128")
+        if (k is None) != (k_weight is None):
+            raise OccfError(f"{what}: keys and their weight come together")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype):
+                raise OccfError(f"{what}: {name} must be [{D}] of {q.dtype}")
+        strides = q.stride()[:3]
+        if k is not None:
+            k = self._heads(what, "k", k, q.dtype, dim=D)
+            if k.shape[:2] != q.shape[:2]:
+                raise OccfError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} need the same batch and length")
+            strides = strides + k.stride()[:3]
+        else:
+            strides = strides + (0, 0, 0)
+        cos, sin, positions, rot, rows, axes, c1, c2, per_b = self._rotation(what, q, cos, sin, positions, axis_dims)
+        w = [None if x is None else x.contiguous() for x in (q_weight, k_weight)]
+        if interleaved:                                                   # a pair is one load
+            even = lambda t: t if t is None or (t.data_ptr() % (2 * t.element_size()) == 0 and
+                                                not any(s % 2 for s in t.stride()[:-1])) \
+                else t.clone(memory_format=torch.contiguous_format)
+            q, k, w = even(q), even(k), [even(x) for x in w]
+            strides = q.stride()[:3] + ((0, 0, 0) if k is None else k.stride()[:3])
+        geom = (ctypes.c_int64 * 17)(B, L, Hq, 0 if k is None else k.shape[2], D, rot, rows, axes, c1, c2, per_b, *strides)
+        return dt, q, k, w, cos, sin, positions, geom
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, cos=None, sin=None, positions=None, eps=1e-6, axis_dims=None,
+                     interleaved=False):
+        """Root-mean-square norm of every head's row of q [B, L, Hq, D] and k [B, L, Hk, D] (any strides with contiguous
+        columns; k and k_weight may be None) with weights [D], and the rotation of the first ``2 * cos.shape[1]`` columns by the
+        table rows of ``position.rotary_table``: pairs (c, c + columns / 2), or neighbours with ``interleaved``.
+        ``positions`` int32 [L] or [B, L] (default 0 .. L - 1), [.., L, axes] where ``axis_dims`` gives the table's columns of each
+        axis.  A position outside the table makes the turned columns of its rows NaN.  cos None: the norm alone.
+        fp32 or bf16 (arithmetic fp32, one rounding) -> new contiguous (q, k)."""
+        dt, q, k, w, cos, sin, positions, geom = self._qk_norm_rope_args("qk_norm_rope", q, k, q_weight, k_weight, cos, sin,
+                                                                        positions, axis_dims, interleaved)
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
+        self._launch_on(q, "occf_qk_norm_rope_fwd", P(q), P(k), P(w[0]), P(w[1]), P(cos), P(sin), P(positions), P(qo), P(ko),
+                        geom, float(eps), int(bool(interleaved)), dt)
+        return qo, ko
+
+    def qk_norm_rope_backward(self, q, k, q_weight, k_weight, dq_out, dk_out, cos=None, sin=None, positions=None, eps=1e-6,
+                              axis_dims=None, interleaved=False):
+        """-> (dq, dk, dq_weight, dk_weight) for the gradients dq_out, dk_out of ``qk_norm_rope``'s outputs"""
+        what = "qk_norm_rope_backward"
+        dt, q, k, w, cos, sin, positions, geom = self._qk_norm_rope_args(what, q, k, q_weight, k_weight, cos, sin, positions,
+                                                                        axis_dims, interleaved, (dq_out, dk_out))
+        for name, x, g in (("dq_out", q, dq_out), ("dk_out", k, dk_out)):
+            if (x is None) != (g is None) or (x is not None and (g.shape != x.shape or g.dtype != q.dtype)):
+                raise OccfError(f"{what}: {name} must have the shape and type of its output")
+        dq_out, dk_out = self._aligned(dq_out.contiguous()), None if k is None else self._aligned(dk_out.contiguous())
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dqw = torch.empty_like(w[0])
+        dkw = None if k is None else torch.empty_like(w[1])
+        ws = self._ws(self.lib.occf_qk_norm_rope_bwd_workspace(q.shape[3]), q.device)
+        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
+        self._launch_on(q, "occf_qk_norm_rope_bwd", P(q), P(k), P(w[0]), P(w[1]), P(cos), P(sin), P(positions), P(dq_out),
+                        P(dk_out), P(dq), P(dk), P(dqw), P(dkw), P(ws), geom, float(eps), int(bool(interleaved)), dt)
+        return dq, dk, dqw, dkw
+
+    @staticmethod
+    def _aligned(t):
+        """``t`` itself where its rows can be read 16 bytes at a time, else a copy"""
+        per16 = 16 // t.element_size()
+        if t.data_ptr() % 16 or any(s % per16 for s in t.stride()[:-1]):
+            return t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    def _rel_attention_args(self, what, q, k, v, table, buckets, scale, causal, lens, grads=()):
+        dt = self._on_device(what, q, k, v, table, buckets.lut, *lens, *grads)
+        q = self._heads(what, "q", q, q.dtype)
+        B, Lq, Hq, D = q.shape
+        k, v = self._heads(what, "k", k, q.dtype, dim=D), self._heads(what, "v", v, q.dtype, dim=D)
+        Lk, Hk = k.shape[1], k.shape[2]
+        if k.shape != v.shape or k.shape[0] != B or Hq % Hk:
+            raise OccfError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: k and v alike, the key heads "
+                            "divide the query heads")
+        if D % 8 or D > 128:
+            raise OccfError(f"{what}: head dim {D} must be a multiple of 8, at most 128")
+        if tuple(table.shape) != (buckets.num_buckets, Hq) or table.dtype != q.dtype:
+            raise OccfError(f"{what}: table must be [{buckets.num_buckets}, {Hq}] of {q.dtype}, got {tuple(table.shape)} of "
+                            f"{table.dtype}")
+        for name, t in zip(("q_lens", "k_lens", "q_start"), lens):
+            if t is not None and (tuple(t.shape) != (B,) or t.dtype != self.i32):
+                raise OccfError(f"{what}: {name} must be int32 [{B}]")
+        scale = float(D) ** -0.5 if scale is None else float(scale)
+        if not 0.0 < scale < float("inf"):
+            raise OccfError(f"{what}: scale {scale} must be positive")
+        q, k, v = self._aligned(q), self._aligned(k), self._aligned(v)
+        geom = (ctypes.c_int64 * 17)(B, Lq, Lk, Hq, Hk, D, buckets.num_buckets, buckets.radius, *q.stride()[:3],
+                                     *k.stride()[:3], *v.stride()[:3])
+        return dt, q, k, v, table.contiguous(), tuple(None if t is None else t.contiguous() for t in lens), scale, geom
+
+    def rel_attention(self, q, k, v, table, buckets, scale=None, causal=False, q_lens=None, k_lens=None, q_start=None,
+                      return_lse=False):
+        """softmax(scale q k^T + table[bucket(j - p_i)]) v with p_i = q_start[b] + i: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D]
+        (any strides with contiguous columns; query head h reads key head h // (Hq / Hk)), table [buckets, Hq] the learned bias,
+        ``buckets`` a ``position.RelativeBuckets``.  Rows i < q_lens[b] see the keys j < k_lens[b], with ``causal`` those at
+        j <= p_i; other rows, and rows that see no key, are zeros.  A table entry at or below -1e30 takes its bucket out.
+        One query of a sequence that grows: q_start = k_lens - 1.  fp32 or bf16 -> [B, Lq, Hq, D]; with ``return_lse`` also the
+        rows' base-2 logarithms of the sum of exponentials, fp32 [B, Hq, Lq], for ``rel_attention_backward``.
+        bf16: probabilities are rounded to bf16 before the product with v (their sum is not)."""
+        dt, q, k, v, table, lens, scale, geom = self._rel_attention_args("rel_attention", q, k, v, table, buckets, scale, causal,
+                                                                        (q_lens, k_lens, q_start))
+        B, Lq, Hq, _ = q.shape
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, Hq, Lq), dtype=self.f32, device=q.device) if return_lse else None
+        need = self.lib.occf_rel_attn_workspace(geom, dt)
+        if need < 0:
+            raise OccfError(f"rel_attention: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        ws = torch.empty((need,), dtype=self.f32, device=q.device) if need else None
+        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
+        self._launch_on(q, "occf_rel_attn_fwd", P(q), P(k), P(v), P(table), P(buckets.lut), P(lens[0]), P(lens[1]), P(lens[2]),
+                        P(out), P(lse), P(ws), need, geom, scale, int(bool(causal)), dt)
+        return (out, lse) if return_lse else out
+
+    def rel_attention_backward(self, q, k, v, table, buckets, out, lse, dout, scale=None, causal=False, q_lens=None,
+                               k_lens=None, q_start=None):
+        """-> (dq, dk, dv, dtable) for ``rel_attention``'s out, lse and the gradient dout of out; rows that do not count get
+        zeros.  bf16: P and dS are rounded to bf16 before their products, dtable's sums are not; the rows' <dout, out> come
+        from the rounded out."""
+        what = "rel_attention_backward"
+        dt, q, k, v, table, lens, scale, geom = self._rel_attention_args(what, q, k, v, table, buckets, scale, causal,
+                                                                        (q_lens, k_lens, q_start), (out, lse, dout))
+        B, Lq, Hq, _ = q.shape
+        for name, t in (("out", out), ("dout", dout)):
+            if t.shape != q.shape or t.dtype != q.dtype:
+                raise OccfError(f"{what}: {name} must have the shape and type of q")
+        if tuple(lse.shape) != (B, Hq, Lq) or lse.dtype != self.f32:
+            raise OccfError(f"{what}: lse must be fp32 [{B}, {Hq}, {Lq}]")
+        out, dout, lse = self._aligned(out.contiguous()), self._aligned(dout.contiguous()), lse.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dtable = torch.empty_like(table)
+        need = self.lib.occf_rel_attn_bwd_workspace(geom, dt)
+        if need < 0:
+            raise OccfError(f"{what}: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        ws = torch.empty((need,), dtype=self.f32, device=q.device)
+        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
+        self._launch_on(q, "occf_rel_attn_bwd", P(q), P(k), P(v), P(table), P(buckets.lut), P(lens[0]), P(lens[1]), P(lens[2]),
+                        P(out), P(lse), P(dout), P(dq), P(dk), P(dv), P(dtable), P(ws), need, geom, scale,
+                        int(bool(causal)), dt)
+        return dq, dk, dv, dtable
 
     # ------------------------------------------------------------------ img_inputs producer (csrc/pipeline.hip)
     def image_resample(self, img, bounds, kk, out_size, vertical):
