@@ -24,6 +24,11 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-result", "-I", os.path.join(ROOT, "include"), "-I", HERE]
 
 
+# accumulators stay in ordinary registers: the default form moves them to and fro at every branch of the tile loops
+# (700 moves in the backward's kernel at head dim 64)
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for f in ("rel_attn.hip", "rel_attn_bwd.hip")}
+
+
 def abi_hash():
     """crc32 of the C header: compiled into the library (occf_abi_hash) and re-checked at load time, so a
     stale .so can never be called through a newer header's prototypes."""
@@ -48,7 +53,7 @@ def _digest():
     h.update(open(os.path.join(ROOT, "include", "occformer_hip.h"), "rb").read())
     # (flags without the checkout's absolute path: the digest identifies the SOURCES -- profiles/*_pmc_traffic.json is
     # stamped with it on one GPU box and checked on another, where the repository lives under a different path)
-    h.update(" ".join(f.replace(ROOT, "<root>") for f in FLAGS).encode())
+    h.update(" ".join(f.replace(ROOT, "<root>") for f in FLAGS + [str(sorted(FILE_FLAGS.items()))]).encode())
     return h.hexdigest()
 
 
@@ -63,7 +68,7 @@ def build(force=False, verbose=True):
 
     def compile_one(src):
         obj = os.path.join(OBJ, src.replace(".hip", ".o"))
-        cmd = [HIPCC, *FLAGS, f"-DOCCF_ABI_HASH={abi_hash()}", "-c", os.path.join(HERE, src), "-o", obj]
+        cmd = [HIPCC, *FLAGS, *FILE_FLAGS.get(src, []), f"-DOCCF_ABI_HASH={abi_hash()}", "-c", os.path.join(HERE, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"hipcc failed for {src}:\n{r.stderr}")

@@ -37,6 +37,10 @@ template <class T> struct RaType;
 template <> struct RaType<float> { static constexpr int NT = 3; };
 template <> struct RaType<ra_bf16> { static constexpr int NT = 1; };
 
+// waves a SIMD that the backward kernels are compiled for: two where their accumulators, fixed operands and tiles in flight fit
+// 256 registers, else one with 512
+#define RA_WAVES_PER_SIMD(T, DP) (DP <= (RaType<T>::NT == 3 ? 32 : 64) ? 2 : 1)
+
 struct RaParams {
   const void *q, *k, *v, *table, *out, *dout;
   const int32_t *lut, *q_lens, *k_lens, *q_start;
@@ -269,6 +273,34 @@ __device__ __forceinline__ void ra_fill_bias(float* lut, const RaParams& p, int 
   }
 }
 
+// Bias and mask of a lane's 16 raw scores s, in place.  The biased base-2 score of entry r is then fma(s[r], ce, be): a tile
+// further than R from the diagonal keeps its raw products (ce = c, be = the outermost bucket's bias), one near it gets the
+// bias added here (ce = 1, be = 0).  `bl`: the bias of entry 0, STEP the sign of the distance along the 16 rows
+// (rows = keys: +1, rows = queries: -1).  The conditions are wave-uniform; the whole tile is one branch each.
+template <int STEP, class Hide>
+__device__ __forceinline__ void ra_bias_mask(f32x16& s, const float* bl, bool near, float far, bool mask, float c, float& ce,
+                                             float& be, Hide hide) {
+  ce = c;
+  be = far;
+  if (near) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], c, bl[STEP * ((r & 3) + 8 * (r >> 2))]);
+    ce = 1.f;
+    be = 0.f;
+  }
+  if (mask) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = hide((r & 3) + 8 * (r >> 2)) ? -INFINITY : s[r];
+  }
+}
+
+__device__ __forceinline__ f32x16 ra_splat16(float x) {
+  f32x16 z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = x;
+  return z;
+}
+
 // rows of sequence b that count: queries [0, nq), keys [0, nk), position of query 0
 __device__ __forceinline__ void ra_lengths(const RaParams& p, int b, int& nq, int& nk, int& start) {
   nq = p.q_lens ? occf_clampi(p.q_lens[b], p.Lq) : p.Lq;
@@ -283,8 +315,9 @@ static int ra_check(const int64_t* g, int dtype) {
   if (!g || (dtype != 0 && dtype != 1)) return OCCF_EINVAL;
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6], R = g[7];
   if (B <= 0 || Lq <= 0 || Lk <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || D < 8 || D > 128 || D % 8) return OCCF_ESHAPE;
-  if (nb < 1 || nb > 128 || R < 1 || R > 1024) return OCCF_ESHAPE;
-  if (Lk > (1L << 29) || Lq > (1L << 29) || B * Hq * ((Lq + 31) / 32) >= 2147483647L || B * Hk * ((Lk + 127) / 128) >= 2147483647L)
+  if (nb < 1 || nb > 128 || R < 1 || R > 512) return OCCF_ESHAPE;
+  if (Lk > (1L << 29) || Lq > (1L << 29) || B * Hq * ((Lq + 31) / 32) * 16 >= 2147483647L ||
+      B * Hk * ((Lk + 127) / 128) * 16 >= 2147483647L)
     return OCCF_ESHAPE;
   if (Lq * (Hq / Hk) >= (1L << 30) || B * Hk * ((Lq * (Hq / Hk) + 31) / 32) * 64 >= 2147483647L) return OCCF_ESHAPE;
   const long per16 = dtype == 0 ? 4 : 8;
@@ -293,8 +326,8 @@ static int ra_check(const int64_t* g, int dtype) {
   return 0;
 }
 
-template <class K>
-static int ra_launch(K kernel, dim3 grid, int threads, size_t lds, void* stream, const RaParams& p) {
+template <class K, class P>
+static int ra_launch(K kernel, dim3 grid, int threads, size_t lds, void* stream, const P& p) {
   if (lds > 160 * 1024) return OCCF_ESHAPE;
 #ifndef OCCF_EMU
   if (lds > 65536) {

@@ -14,33 +14,11 @@
 
 #define RA_EXCEED 8.0f          // the running maximum follows only when a tile exceeds it by 2^8: p <= 256, sums stay fp32
 
-// one 32-key score tile of a lane: t (base 2, biased, masked) from the raw products s; returns its maximum
-// jl = j0 + 4 lk; pi = position of this lane's query
-template <bool MASK>
-__device__ __forceinline__ float ra_scores(f32x16& s, const float* lut, const RaParams& p, int j0, int pi, int lk, int nk,
-                                           bool near, float far) {
-  float mx = -INFINITY;
-  const int jl = j0 + 4 * lk;
-  const float* bl = lut + (near ? jl - pi + p.R + RA_PAD : 0);
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int o = (r & 3) + 8 * (r >> 2);
-    float t = near ? fmaf(s[r], p.c, bl[o]) : fmaf(s[r], p.c, far);
-    if (MASK) {
-      const int j = jl + o;
-      if (j >= nk || (p.causal && j > pi)) t = -INFINITY;
-    }
-    s[r] = t;
-    mx = fmaxf(mx, t);
-  }
-  return mx;
-}
-
 // ---------------------------------------------------------------------------------------------------------------------
 // Many queries: a workgroup owns 128 queries of one head, a wave 32 of them (a lane one query: its running maximum and sum
 // are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.
 template <class T, int DP, int KT>
-__global__ void __launch_bounds__(256) rel_attn_fwd_kernel(RaParams p) {
+__global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) rel_attn_fwd_kernel(RaParams p) {
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
   constexpr int NB = KT * DP / 16, NU = (NB + 255) / 256;               // 4 x 4 blocks of a tile, and a thread's share
   OCCF_DYN_SMEM(smem);
@@ -51,8 +29,11 @@ __global__ void __launch_bounds__(256) rel_attn_fwd_kernel(RaParams p) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
   const int nqt = (p.Lq + 127) / 128;
   unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  const int qt = nqt - 1 - (int)(bid % nqt);            // causal: the longest rows first
+  // causal rows differ in length: every other head walks them the other way, so that the workgroups that one compute unit
+  // holds (a fixed step apart) add up to the same work
+  const int back = (int)(bid % nqt);
   bid /= nqt;
+  const int qt = bid & 1 ? back : nqt - 1 - back;
   const int h = (int)(bid % p.Hq), b = (int)(bid / p.Hq);
   const int hk = h / (p.Hq / p.Hk);
   int nq, nk, start;
@@ -125,16 +106,19 @@ __global__ void __launch_bounds__(256) rel_attn_fwd_kernel(RaParams p) {
       for (int ks = 0; ks < KS; ++ks)
         s[sub] = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s[sub]);
     }
-    float mx = -INFINITY;
+    float mx = -INFINITY, ce[KT / 32], be[KT / 32];
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);           // tile distances: rel0 - 31 .. rel0 + 31
+      const int jl = j0 + 4 * lk;
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
-      const float far = lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD];
-      const bool mask = j0 + 32 > kend || (p.causal && j0 + 31 > start + i0);
-      const float x = mask ? ra_scores<true>(s[sub], lut, p, j0, pi, lk, kend, near, far)
-                           : ra_scores<false>(s[sub], lut, p, j0, pi, lk, kend, near, far);
-      mx = fmaxf(mx, x);
+      ra_bias_mask<1>(s[sub], lut + (near ? jl - pi + p.R + RA_PAD : 0), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+                      j0 + 32 > kend || (p.causal && rel0 + 31 > 0), p.c, ce[sub], be[sub],
+                      [&](int o) { return jl + o >= kend || (p.causal && jl + o > pi); });
+      float x = s[sub][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) x = fmaxf(x, s[sub][r]);
+      mx = fmaxf(mx, fmaf(x, ce[sub], be[sub]));
     }
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (__ballot(mx > m + RA_EXCEED)) {
@@ -151,9 +135,10 @@ __global__ void __launch_bounds__(256) rel_attn_fwd_kernel(RaParams p) {
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       float pv[16];
+      const float off = be[sub] - mref;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        pv[r] = ra_exp2(s[sub][r] - mref);
+        pv[r] = ra_exp2(fmaf(s[sub][r], ce[sub], off));
         l += pv[r];
       }
 #pragma unroll
@@ -198,7 +183,7 @@ struct RaFew {
 };
 
 template <class T, int DP>
-__global__ void __launch_bounds__(256) rel_attn_few_kernel(RaParams p) {
+__global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 32 ? 2 : 1) rel_attn_few_kernel(RaParams p) {
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
   constexpr int NB = 2 * DP, NV = (NB + 63) / 64;                        // 4 x 4 blocks of 32 value rows, and a lane's share
   OCCF_DYN_SMEM(smem);

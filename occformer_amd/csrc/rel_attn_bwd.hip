@@ -4,70 +4,63 @@
 //   P = exp2(t - lse),  dV = P^T dO,  dP = dO V^T,  delta_i = dO_i . O_i,  dS = P (dP - delta)
 //   dQ = scale dS K,    dK = scale dS^T Q,    dT[b, h] = sum of dS over the pairs whose distance is in bucket b
 //
-// Two kernels, one an operand orientation, so that P and dS never leave registers and every gradient is written once, by one
-// wave, in a fixed order (no atomics):
-//   rel_attn_dq_kernel   a wave owns 32 queries (lane = query) and walks the keys:  S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T;
-//                        also leaves delta for the other kernel and the distances' sums of dS
+// Two kernels, one an operand orientation, so that P and dS never leave registers and every sum has a fixed order (no atomics):
+//   rel_attn_dq_kernel   a wave owns 32 queries (lane = query) and walks the keys:  S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   rel_attn_dkv_kernel  a wave owns 32 keys (lane = key) and walks the queries of every head that shares them:
-//                        S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+//                        S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS, and the distances' sums of dS
 // The scores are formed twice: 7 products instead of 5, where a single pass would have to add dQ up across workgroups.
+// -lse / c and -delta are the accumulators' first values, so that neither costs an instruction a score.
+//
+// delta: a row of dS sums to zero, but <dO, O> of an O rounded to bf16 (whose P was rounded too) is off by a few 2^-9, and the
+// bias' gradient, sums of dS that nearly cancel, shows it (3.5e-3 of error where its own rounding is 1.7e-3).  The row sums of
+// the dS so formed ARE that error (P sums to one), so the first kernel adds them to the delta that the second one reads, and
+// takes (row sum) x (P K) off its own dQ: one product more, bf16 only; an fp32 O leaves nothing to correct in dQ.
+//
+// Both walks are cut into `splits` where whole ones would not fill the card; rel_attn_finish_kernel adds the parts up in order.
 #include "rel_attn.h"
 #include "../../include/occformer_hip.h"
 
 #define RA_DLD 33               // row of the 32 x 32 tile whose diagonals are summed
 
-// P of a lane's 16 scores: exponent base-2 t - lse, zero where the pair does not count
-template <bool MASK>
-__device__ __forceinline__ void ra_probs(f32x16& s, const float* bl, bool near, float far, float c, float lse, int jl, int pi,
-                                         int nk, int causal) {
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int o = (r & 3) + 8 * (r >> 2);
-    float t = near ? fmaf(s[r], c, bl[o] - lse) : fmaf(s[r], c, far - lse);
-    if (MASK) {
-      const int j = jl + o;
-      if (j >= nk || (causal && j > pi)) t = -INFINITY;
-    }
-    s[r] = ra_exp2(t);
-  }
-}
+struct RaBwd {
+  RaParams a;
+  void* dtable;
+  float *eps, *dq_part, *pk_part, *dk_part, *dv_part, *tab_part;
+  int qsplit, ksplit;            // parts of the keys a query's walk is cut into; parts of the queries a key's
+};
 
-template <class T, int DP, int KT, int NW>
+template <class T, int DP, int KT>
 struct RaDq {
   static constexpr int NT = RaType<T>::NT;
   static constexpr int images = NT * (2 * RaRow<DP>::bytes(KT) + RaTrans<KT>::bytes(DP));
-  static size_t bytes(int R) {
-    const size_t n = 2 * (size_t)R + 1 + 2 * RA_PAD;
-    return images + 4 * (n + NW * n + NW * 32 * RA_DLD);
-  }
+  static size_t bytes(int R) { return images + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
 };
 
 template <class T, int DP, int KT, int NW>
-__global__ void __launch_bounds__(NW * 64) rel_attn_dq_kernel(RaParams p) {
+__global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq_kernel(RaBwd g) {
+  const RaParams& p = g.a;
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, QW = NW * 32;
   constexpr int NB = KT * DP / 16, NU = (NB + TH - 1) / TH;
+  constexpr bool PK = NT == 1;
   OCCF_DYN_SMEM(smem);
   char* img_k = smem;
   char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
   char* img_kt = img_v + NT * RaRow<DP>::bytes(KT);
-  const int nl = 2 * p.R + 1 + 2 * RA_PAD;
   float* lut = (float*)(img_kt + NT * RaTrans<KT>::bytes(DP));
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
-  float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
-  float* dsum = sums + wave * nl;
-  float* tile = sums + NW * nl + wave * 32 * RA_DLD;
 
   const int nqt = (p.Lq + QW - 1) / QW;
   unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  const unsigned wg = bid;
-  const int qt = nqt - 1 - (int)(bid % nqt);
+  const int back = (int)(bid % nqt);
   bid /= nqt;
+  const int qt = bid & 1 ? back : nqt - 1 - back;        // (see rel_attn_fwd_kernel)
+  const int split = (int)(bid % g.qsplit);
+  bid /= g.qsplit;
   const int h = (int)(bid % p.Hq), b = (int)(bid / p.Hq);
   const int hk = h / (p.Hq / p.Hk);
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
   ra_fill_bias<T>(lut, p, h, tid, TH);
-  for (int t = tid; t < NW * nl; t += TH) sums[t] = 0.f;
 
   const int i0 = qt * QW + wave * 32, i = i0 + li, pi = start + i;
   const bool live = i < nq;
@@ -92,7 +85,8 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dq_kernel(RaParams p) {
   const long stat = ((long)b * p.Hq + h) * p.Lq + ic;
   float lse = live ? p.lse[stat] : INFINITY;
   if (lse == -INFINITY) lse = INFINITY;                  // no key: P = 0
-  if (i < p.Lq && lk == 0) p.delta[stat] = delta;
+  if (i < p.Lq && lk == 0 && split == 0) p.delta[stat] = delta;
+  const f32x16 s_first = ra_splat16(-lse / p.c), dp_first = ra_splat16(-delta);
 
   int kend = nk;
   if (p.causal) {
@@ -103,22 +97,26 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dq_kernel(RaParams p) {
   const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
   const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
 
-  f32x16 acc[DT];
+  f32x16 acc[DT], pk[PK ? DT : 1];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
-  float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
+#pragma unroll
+  for (int dt = 0; dt < (PK ? DT : 1); ++dt) pk[dt] = ra_zero16();
+  float eps = 0.f;
 
   RaBlk<T> rk[NU], rv[NU];
   const int ntile = (kend + KT - 1) / KT;
-  if (ntile > 0) {
+  const int t0 = (int)((long)ntile * split / g.qsplit), t1 = (int)((long)ntile * (split + 1) / g.qsplit);
+  auto load = [&](int k0) {
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T, DP>(rk[n], kb, p.ksl, 0, kend, p.D, tid + n * TH);
-      ra_load_blk<T, DP>(rv[n], vb, p.vsl, 0, kend, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(rk[n], kb, p.ksl, k0, kend, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(rv[n], vb, p.vsl, k0, kend, p.D, tid + n * TH);
     }
-  }
-  for (int kt = 0; kt < ntile; ++kt) {
+  };
+  if (t0 < t1) load(t0 * KT);
+  for (int kt = t0; kt < t1; ++kt) {
     const int k0 = kt * KT;
     __syncthreads();
 #pragma unroll
@@ -132,138 +130,81 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dq_kernel(RaParams p) {
       ra_store_row<NT, DP, KT>(img_v, w, tid + n * TH);
     }
     __syncthreads();
-    if (kt + 1 < ntile) {
-#pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        if (NB % TH && tid + n * TH >= NB) break;
-        ra_load_blk<T, DP>(rk[n], kb, p.ksl, k0 + KT, kend, p.D, tid + n * TH);
-        ra_load_blk<T, DP>(rv[n], vb, p.vsl, k0 + KT, kend, p.D, tid + n * TH);
-      }
-    }
+    if (kt + 1 < t1) load(k0 + KT);
     if (i0 >= nq) continue;                              // wave-uniform
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= kend || (p.causal && rel0 > 31)) continue;
-      f32x16 s = ra_zero16(), dp = ra_zero16();
+      f32x16 s = s_first, dp = dp_first;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s);
         dp = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_v, sub * 32, ks, li, lk), of[ks], dp);
       }
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
-      const float far = lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD];
       const int jl = j0 + 4 * lk;
-      const float* bl = lut + (near ? jl - pi + p.R + RA_PAD : 0);
-      if (j0 + 32 > kend || (p.causal && rel0 + 31 > 0))
-        ra_probs<true>(s, bl, near, far, p.c, lse, jl, pi, kend, p.causal);
-      else
-        ra_probs<false>(s, bl, near, far, p.c, lse, jl, pi, kend, p.causal);
-      float ds[16];
+      float ce, be;
+      ra_bias_mask<1>(s, lut + (near ? jl - pi + p.R + RA_PAD : 0), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+                      j0 + 32 > kend || (p.causal && rel0 + 31 > 0), p.c, ce, be,
+                      [&](int o) { return jl + o >= kend || (p.causal && jl + o > pi); });
+      float ds[16], pv[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = s[r] * (dp[r] - delta);
-      if (near) {
-        // sums along the diagonals: lane e adds the pairs at distance rel0 + e - 31 (63 of them), in LDS of the wave's own
-        RA_WAVE_SYNC();
-#pragma unroll
-        for (int r = 0; r < 16; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * RA_DLD + li] = ds[r];
-        RA_WAVE_SYNC();
-        float x = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < 32; ++q) {
-          const int row = q + lane - 31;
-          if (row >= 0 && row < 32) x += tile[row * RA_DLD + q];
-        }
-        const int at = rel0 + lane - 31 + p.R + RA_PAD;
-        if (lane < 63) dsum[at] += x;
-      } else {
-        float x = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x += ds[r];
-        if (rel0 > 0) above += x;
-        else below += x;
+      for (int r = 0; r < 16; ++r) {
+        pv[r] = ra_exp2(fmaf(s[r], ce, be));
+        ds[r] = pv[r] * dp[r];
+        eps += ds[r];
       }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        const RaFrag<NT> df = ra_pack8<NT>(ds + s2 * 8);
+        const RaFrag<NT> df = ra_pack8<NT>(ds + s2 * 8), pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-          acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, KT>(img_kt, dt * 32, sub * 2 + s2, li, lk), df, acc[dt]);
+        for (int dt = 0; dt < DT; ++dt) {
+          const RaFrag<NT> kt_f = ra_read_trans<NT, DP, KT>(img_kt, dt * 32, sub * 2 + s2, li, lk);
+          acc[dt] = ra_mm<NT>(kt_f, df, acc[dt]);
+          if (PK) pk[dt] = ra_mm<NT>(kt_f, pf, pk[dt]);
+        }
       }
     }
   }
-  if (i < p.Lq) {
-    T* row = (T*)p.dq + orow;
+  eps += __shfl_xor(eps, 32);
+  if (i >= p.Lq) return;
+  if (lk == 0) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;
+  const long part = (long)split * p.B * p.Lq * p.Hq * p.D + orow;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = dt * 32 + 8 * g + 4 * lk;
-        if (d < p.D)
-          ra_store4(row + d, acc[dt][4 * g] * p.scale, acc[dt][4 * g + 1] * p.scale, acc[dt][4 * g + 2] * p.scale,
-                    acc[dt][4 * g + 3] * p.scale);
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + 8 * q + 4 * lk;
+      if (d >= p.D) continue;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = acc[dt][4 * q + e];
+      if (g.qsplit > 1) {
+        ra_store4(g.dq_part + part + d, x[0], x[1], x[2], x[3]);
+        if (PK) ra_store4(g.pk_part + part + d, pk[dt][4 * q], pk[dt][4 * q + 1], pk[dt][4 * q + 2], pk[dt][4 * q + 3]);
+        continue;
       }
-  }
+      if (PK) {
 #pragma unroll
-  for (int mm = 32; mm > 0; mm >>= 1) {
-    below += __shfl_xor(below, mm);
-    above += __shfl_xor(above, mm);
-  }
-  RA_WAVE_SYNC();
-  if (lane == 0) {
-    dsum[0] += below;
-    dsum[nl - 1] += above;
-  }
-  __syncthreads();
-  // this workgroup's sums by clamped distance, waves in order, then the columns beyond either end
-  float* part = p.part + (long)wg * (2 * p.R + 1);
-  for (int t = tid; t < 2 * p.R + 1; t += TH) {
-    const int lo = t == 0 ? 0 : t + RA_PAD, hi = t == 2 * p.R ? nl : t + RA_PAD + 1;
-    float x = 0.f;
-    for (int a = lo; a < hi; ++a)
-#pragma unroll
-      for (int w = 0; w < NW; ++w) x += sums[w * nl + a];
-    part[t] = x;
-  }
-}
-
-// dT of one head: the workgroups' sums by distance in order, then every bucket's distances in order
-template <class T>
-__global__ void __launch_bounds__(1024) rel_attn_dtable_kernel(RaParams p, T* dtable, int nqt) {
-  OCCF_DYN_SMEM(smem);
-  const int n = 2 * p.R + 1, h = blockIdx.x, tid = threadIdx.x;
-  float* sum = (float*)smem;                             // [n]
-  int* lut = (int*)(sum + n);                            // [n]
-  for (int t = tid; t < n; t += 1024) {
-    float x = 0.f;
-    for (int b = 0; b < p.B; ++b) {
-      const float* src = p.part + ((long)b * p.Hq + h) * nqt * n + t;
-#pragma unroll 8
-      for (int q = 0; q < nqt; ++q) x += src[(long)q * n];
+        for (int e = 0; e < 4; ++e) x[e] = fmaf(-eps, pk[dt][4 * q + e], x[e]);
+      }
+      ra_store4((T*)p.dq + orow + d, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
     }
-    sum[t] = x;
-    lut[t] = occf_clampi(p.lut[t], p.nb - 1);
-  }
-  __syncthreads();
-  for (int b = tid; b < p.nb; b += 1024) {
-    float x = 0.f;
-    for (int t = 0; t < n; ++t)
-      if (lut[t] == b) x += sum[t];
-    T* dst = dtable + (long)b * p.Hq + h;
-    if constexpr (sizeof(T) == 4) *dst = x;
-    else *dst = (T)occf_bf16_1(x);
-  }
 }
 
-template <class T, int DP, int QT>
+template <class T, int DP, int QT, int NW>
 struct RaDkv {
   static constexpr int NT = RaType<T>::NT;
   static constexpr int images = 2 * NT * (RaRow<DP>::bytes(QT) + RaTrans<QT>::bytes(DP));
-  static size_t bytes(int R) { return images + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD + 2 * QT); }
+  static size_t bytes(int R) {
+    return images + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + 2 * QT + NW * 32 * RA_DLD);
+  }
 };
 
 template <class T, int DP, int QT, int NW>
-__global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
+__global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dkv_kernel(RaBwd g) {
+  const RaParams& p = g.a;
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, KW = NW * 32;
   constexpr int NB = QT * DP / 16, NU = (NB + TH - 1) / TH;
   OCCF_DYN_SMEM(smem);
@@ -271,17 +212,24 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
   char* img_o = img_q + NT * RaRow<DP>::bytes(QT);
   char* img_qt = img_o + NT * RaRow<DP>::bytes(QT);
   char* img_ot = img_qt + NT * RaTrans<QT>::bytes(DP);
-  float* s_lse = (float*)(img_ot + NT * RaTrans<QT>::bytes(DP));
+  float* s_lse = (float*)(img_ot + NT * RaTrans<QT>::bytes(DP));       // first values of the accumulators' rows
   float* s_delta = s_lse + QT;
-  float* lut = s_delta + QT;
+  float* tiles = s_delta + QT;
+  float* lut = tiles + NW * 32 * RA_DLD;
+  const int nl = 2 * p.R + 1 + 2 * RA_PAD;
+  float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  float* dsum = sums + wave * nl;
+  float* tile = tiles + wave * 32 * RA_DLD;
 
-  const int nkt = (p.Lk + KW - 1) / KW;
+  const int nkt = (p.Lk + KW - 1) / KW, G = p.Hq / p.Hk;
   unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  const int kt = (int)(bid % nkt);                       // causal: the first keys have the most queries
+  const int back = (int)(bid % nkt);
   bid /= nkt;
+  const int kt = bid & 1 ? nkt - 1 - back : back;
+  const int split = (int)(bid % g.ksplit);
+  bid /= g.ksplit;
   const int hk = (int)(bid % p.Hk), b = (int)(bid / p.Hk);
-  const int G = p.Hq / p.Hk;
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
 
@@ -305,6 +253,16 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
     first = at > 0 ? at / QT * QT : 0;
   }
   const int ntile = kt * KW >= nk || first >= nq ? 0 : (nq - first + QT - 1) / QT;
+  // steps: the query tiles of every head of the group, in order; this workgroup's share of them
+  const int t0 = (int)((long)ntile * G * split / g.ksplit), t1 = (int)((long)ntile * G * (split + 1) / g.ksplit);
+  float* tab = g.tab_part + ((((long)b * p.Hk + hk) * g.ksplit + split) * nkt + kt) * G * p.nb;       // [G][nb]
+
+  for (int t = tid; t < NW * nl; t += TH) sums[t] = 0.f;
+  // heads that this share does not touch
+  for (int t = tid; t < G * p.nb; t += TH) {
+    const int hg = t / p.nb;
+    if (t0 >= t1 || hg < t0 / ntile || hg > (t1 - 1) / ntile) tab[t] = 0.f;
+  }
 
   f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -312,6 +270,7 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
     dk[dt] = ra_zero16();
     dv[dt] = ra_zero16();
   }
+  float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
   RaBlk<T> rq[NU], ro[NU];
   float nlse = 0.f, ndelta = 0.f;
   auto load = [&](int step) {
@@ -327,17 +286,21 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
     if (tid < QT) {
       const int i = r0 + tid;
       const long stat = ((long)b * p.Hq + h) * p.Lq + i;
-      nlse = i < nq ? p.lse[stat] : INFINITY;
-      if (nlse == -INFINITY) nlse = INFINITY;
-      ndelta = i < nq ? p.delta[stat] : 0.f;
+      nlse = INFINITY;
+      ndelta = 0.f;
+      if (i < nq) {
+        const float x = p.lse[stat];
+        nlse = x == -INFINITY ? INFINITY : x;
+        ndelta = p.delta[stat];
+        for (int s = 0; s < g.qsplit; ++s) ndelta += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
+      }
     }
   };
-  const int steps = ntile * G;
-  if (steps > 0) load(0);
-  for (int step = 0; step < steps; ++step) {
-    const int r0 = first + (step % ntile) * QT;
+  if (t0 < t1) load(t0);
+  for (int step = t0; step < t1; ++step) {
+    const int hg = step / ntile, r0 = first + (step - hg * ntile) * QT;
     __syncthreads();
-    if (step % ntile == 0) ra_fill_bias<T>(lut, p, hk * G + step / ntile, tid, TH);
+    if (step == t0 || step == hg * ntile) ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
@@ -350,48 +313,64 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
       ra_store_trans<NT, DP, QT>(img_ot, w, tid + n * TH);
     }
     if (tid < QT) {
-      s_lse[tid] = nlse;
-      s_delta[tid] = ndelta;
+      s_lse[tid] = -nlse / p.c;
+      s_delta[tid] = -ndelta;
     }
     __syncthreads();
-    if (step + 1 < steps) load(step + 1);
-    if (j0 >= nk) continue;                              // wave-uniform
+    if (step + 1 < t1) load(step + 1);
 #pragma unroll
     for (int sub = 0; sub < QT / 32; ++sub) {
       const int i0 = r0 + sub * 32, rel0 = j0 - (start + i0);
-      if (i0 >= nq || (p.causal && rel0 > 31)) continue;
-      f32x16 s = ra_zero16(), dp = ra_zero16();
+      if (j0 >= nk || i0 >= nq || (p.causal && rel0 > 31)) continue;      // wave-uniform
+      f32x16 s, dp;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 x = *(const float4*)(s_lse + sub * 32 + 8 * q + 4 * lk);
+        const float4 y = *(const float4*)(s_delta + sub * 32 + 8 * q + 4 * lk);
+        s[4 * q] = x.x; s[4 * q + 1] = x.y; s[4 * q + 2] = x.z; s[4 * q + 3] = x.w;
+        dp[4 * q] = y.x; dp[4 * q + 1] = y.y; dp[4 * q + 2] = y.z; dp[4 * q + 3] = y.w;
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = ra_mm<NT>(ra_read_row<NT, DP, QT>(img_q, sub * 32, ks, li, lk), kf[ks], s);
         dp = ra_mm<NT>(ra_read_row<NT, DP, QT>(img_o, sub * 32, ks, li, lk), vf[ks], dp);
       }
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
-      const float far = lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD];
-      const bool mask = j0 + 32 > nk || (p.causal && rel0 + 31 > 0);
-      const int il = i0 + 4 * lk;                        // rows il + (r & 3) + 8 (r >> 2)
-      const float* bl = lut + (near ? j - (start + il) + p.R + RA_PAD : 32);
-      float ds[16];
+      const int pl = start + i0 + 4 * lk;                // position of row 0 of this lane
+      float ce, be;
+      ra_bias_mask<-1>(s, lut + (near ? j - pl + p.R + RA_PAD : 32), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+                       j0 + 32 > nk || (p.causal && rel0 + 31 > 0), p.c, ce, be,
+                       [&](int o) { return !live || (p.causal && j > pl + o); });
+      float ds[16], pv[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const float4 ls = *(const float4*)(s_lse + sub * 32 + 8 * g + 4 * lk);
-        const float4 de = *(const float4*)(s_delta + sub * 32 + 8 * g + 4 * lk);
-        const float lse4[4] = {ls.x, ls.y, ls.z, ls.w}, del4[4] = {de.x, de.y, de.z, de.w};
+      for (int r = 0; r < 16; ++r) {
+        pv[r] = ra_exp2(fmaf(s[r], ce, be));
+        ds[r] = pv[r] * dp[r];
+      }
+      if (near) {
+        // sums along the diagonals: lane e adds the pairs at distance rel0 + e - 31 (63 of them), in LDS of the wave's own
+        RA_WAVE_SYNC();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e, o = e + 8 * g;
-          float t = fmaf(s[r], p.c, (near ? bl[-o] : far) - lse4[e]);
-          if (mask && (!live || (p.causal && j > start + il + o))) t = -INFINITY;
-          s[r] = ra_exp2(t);
-          ds[r] = s[r] * (dp[r] - del4[e]);
+        for (int r = 0; r < 16; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * RA_DLD + li] = ds[r];
+        RA_WAVE_SYNC();
+        float x = 0.f;
+#pragma unroll 8
+        for (int q = 0; q < 32; ++q) {
+          const int col = q + lane - 31;
+          const float y = tile[q * RA_DLD + occf_clampi(col, 31)];
+          x += col >= 0 && col < 32 ? y : 0.f;
         }
+        if (lane < 63) dsum[rel0 + lane - 31 + p.R + RA_PAD] += x;
+      } else {
+        float x = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x += ds[r];
+        if (rel0 > 0) above += x;
+        else below += x;
       }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        float pv[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pv[e] = s[s2 * 8 + e];
-        const RaFrag<NT> pf = ra_pack8<NT>(pv), df = ra_pack8<NT>(ds + s2 * 8);
+        const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8), df = ra_pack8<NT>(ds + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           dv[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_ot, dt * 32, sub * 2 + s2, li, lk), pf, dv[dt]);
@@ -399,43 +378,185 @@ __global__ void __launch_bounds__(NW * 64) rel_attn_dkv_kernel(RaParams p) {
         }
       }
     }
+    if (step + 1 == t1 || step + 1 == (hg + 1) * ntile) {
+      // a head is done: its distances' sums, waves in order, then the buckets', distances in order
+#pragma unroll
+      for (int mm = 32; mm > 0; mm >>= 1) {
+        below += __shfl_xor(below, mm);
+        above += __shfl_xor(above, mm);
+      }
+      RA_WAVE_SYNC();
+      if (lane == 0) {
+        dsum[0] += below;
+        dsum[nl - 1] += above;
+      }
+      below = above = 0.f;
+      __syncthreads();
+      for (int t = tid; t < nl; t += TH) {
+        float x = sums[t];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+          x += sums[w * nl + t];
+          sums[w * nl + t] = 0.f;
+        }
+        sums[t] = x;
+      }
+      __syncthreads();
+      // `tl` threads a bucket walk every tl-th distance (the columns beyond either end count as the end)
+      int nb2 = 4;
+      while (nb2 < p.nb) nb2 <<= 1;
+      const int tl = TH / nb2, bk = tid / tl, r = tid % tl;
+      float x = 0.f;
+      if (bk < p.nb)
+        for (int t = r; t < nl; t += tl)
+          if (occf_clampi(p.lut[occf_clampi(t - RA_PAD, 2 * p.R)], p.nb - 1) == bk) x += sums[t];
+      for (int mm = 1; mm < tl; mm <<= 1) x += __shfl_xor(x, mm);
+      if (bk < p.nb && r == 0) tab[hg * p.nb + bk] = x;
+      __syncthreads();
+      for (int t = tid; t < nl; t += TH) sums[t] = 0.f;
+    }
   }
   if (j >= p.Lk) return;
-  const float keep = live ? 1.f : 0.f;
   const long out = (((long)b * p.Lk + j) * p.Hk + hk) * p.D;
+  const long part = (long)split * p.B * p.Lk * p.Hk * p.D + out;
+  if (!live) {                                           // keys that do not count
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) dk[dt] = dv[dt] = ra_zero16();
+  }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int d = dt * 32 + 8 * g + 4 * lk;
+    for (int q = 0; q < 4; ++q) {
+      const int d = dt * 32 + 8 * q + 4 * lk;
       if (d >= p.D) continue;
-      const float a = p.scale * keep;
-      ra_store4((T*)p.dk + out + d, dk[dt][4 * g] * a, dk[dt][4 * g + 1] * a, dk[dt][4 * g + 2] * a, dk[dt][4 * g + 3] * a);
-      ra_store4((T*)p.dv + out + d, dv[dt][4 * g] * keep, dv[dt][4 * g + 1] * keep, dv[dt][4 * g + 2] * keep,
-                dv[dt][4 * g + 3] * keep);
+      const f32x16 &x = dk[dt], &y = dv[dt];
+      if (g.ksplit > 1) {
+        ra_store4(g.dk_part + part + d, x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+        ra_store4(g.dv_part + part + d, y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+      } else {
+        ra_store4((T*)p.dk + out + d, x[4 * q] * p.scale, x[4 * q + 1] * p.scale, x[4 * q + 2] * p.scale, x[4 * q + 3] * p.scale);
+        ra_store4((T*)p.dv + out + d, y[4 * q], y[4 * q + 1], y[4 * q + 2], y[4 * q + 3]);
+      }
     }
 }
 
+// The parts in order: the first Hq workgroups make the bias' gradient, then dq and then dk, dv where their walks were cut
+// (four columns a thread).
+template <class T>
+__global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int dq_blocks) {
+  const RaParams& p = g.a;
+  const int tid = threadIdx.x;
+  int blk = blockIdx.x;
+  if (blk < p.Hq) {
+    __shared__ float acc[256];
+    const int G = p.Hq / p.Hk, hk = blk / G, hg = blk % G;
+    int nb2 = 1;
+    while (nb2 < p.nb) nb2 <<= 1;
+    const int b = tid % nb2, r = tid / nb2, lanes = 256 / nb2;
+    const int rows = g.ksplit * nkt;
+    float x = 0.f;
+    if (b < p.nb)
+      for (int s = 0; s < p.B; ++s) {
+        const float* src = g.tab_part + (((long)s * p.Hk + hk) * rows * G + hg) * p.nb + b;
+#pragma unroll 4
+        for (int q = r; q < rows; q += lanes) x += src[(long)q * G * p.nb];
+      }
+    acc[tid] = x;
+    __syncthreads();
+    if (r == 0 && b < p.nb) {
+      x = 0.f;
+      for (int q = 0; q < lanes; ++q) x += acc[q * nb2 + b];
+      T* dst = (T*)g.dtable + (long)b * p.Hq + blk;
+      if constexpr (sizeof(T) == 4) *dst = x;
+      else *dst = (T)occf_bf16_1(x);
+    }
+    return;
+  }
+  blk -= p.Hq;
+  const bool dq = blk < dq_blocks;
+  const long at = ((long)(dq ? blk : blk - dq_blocks) * 256 + tid) * 4;
+  const long n = dq ? (long)p.B * p.Lq * p.Hq * p.D : (long)p.B * p.Lk * p.Hk * p.D;
+  if (at >= n) return;
+  const int splits = dq ? g.qsplit : g.ksplit;
+  const float *pa = dq ? g.dq_part : g.dk_part, *pb = dq ? g.pk_part : g.dv_part;
+  const bool second = !dq || RaType<T>::NT == 1;
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float4 a = *(const float4*)(pa + s * n + at);
+    x[0] += a.x; x[1] += a.y; x[2] += a.z; x[3] += a.w;
+    if (second) {
+      const float4 c = *(const float4*)(pb + s * n + at);
+      y[0] += c.x; y[1] += c.y; y[2] += c.z; y[3] += c.w;
+    }
+  }
+  if (dq) {
+    float eps = 0.f;
+    if (second) {
+      const long row = at / p.D;                         // (b Lq + i) Hq + h
+      const int h = (int)(row % p.Hq);
+      const long bi = row / p.Hq;
+      const long stat = (bi / p.Lq * p.Hq + h) * p.Lq + bi % p.Lq;
+      for (int s = 0; s < splits; ++s) eps += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(-eps, y[e], x[e]) * p.scale;
+    ra_store4((T*)p.dq + at, x[0], x[1], x[2], x[3]);
+  } else {
+    ra_store4((T*)p.dk + at, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
+    ra_store4((T*)p.dv + at, y[0], y[1], y[2], y[3]);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
+// How often the walks are cut: until about four workgroups a compute unit are there, in steps of two or more tiles.
+static void ra_bwd_plan(const int64_t* g, int& qsplit, int& ksplit) {
+  const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
+  const long wq = B * Hq * ((Lq + 127) / 128), wk = B * Hk * ((Lk + 127) / 128);
+  const long mq = (Lk + 127) / 128, mk = (Hq / Hk) * ((Lq + 127) / 128);
+  const auto cut = [](long want, long most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
+  qsplit = wq >= 512 ? 1 : cut(cut(1024 / wq, mq), 16);
+  ksplit = wk >= 512 ? 1 : cut(cut(1024 / wk, mk), 16);
+}
+
+struct RaBwdSizes { long delta, eps, dq, dk, tab; };
+static RaBwdSizes ra_bwd_sizes(const int64_t* g, int dtype, int qsplit, int ksplit) {
+  const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6];
+  RaBwdSizes s;
+  const auto up = [](long n) { return (n + 63) / 64 * 64; };             // parts start on 256 bytes
+  s.delta = up(B * Hq * Lq);
+  s.eps = up(B * Hq * Lq * qsplit);
+  s.dq = qsplit > 1 ? up(B * Lq * Hq * D * qsplit) : 0;
+  s.dk = ksplit > 1 ? up(B * Lk * Hk * D * ksplit) : 0;
+  s.tab = up(B * Hq * ksplit * ((Lk + 127) / 128) * nb);
+  (void)dtype;
+  return s;
+}
+
 template <class T, int DP>
-static int ra_bwd(RaParams& p, void* dtable, void* stream) {
+static int ra_bwd(const RaBwd& g, void* stream) {
   constexpr int NW = 4, KT = RaType<T>::NT == 3 && DP > 64 ? 32 : 64, QT = RaType<T>::NT == 3 ? 32 : 64;
-  const int nqt = (p.Lq + NW * 32 - 1) / (NW * 32), nkt = (p.Lk + NW * 32 - 1) / (NW * 32);
-  int rc = ra_launch(rel_attn_dq_kernel<T, DP, KT, NW>, dim3((unsigned)((long)p.B * p.Hq * nqt)), NW * 64,
-                     RaDq<T, DP, KT, NW>::bytes(p.R), stream, p);
+  const RaParams& p = g.a;
+  const long nqt = (p.Lq + NW * 32 - 1) / (NW * 32), nkt = (p.Lk + NW * 32 - 1) / (NW * 32);
+  int rc = ra_launch(rel_attn_dq_kernel<T, DP, KT, NW>, dim3((unsigned)(p.B * p.Hq * nqt * g.qsplit)), NW * 64,
+                     RaDq<T, DP, KT>::bytes(p.R), stream, g);
   if (rc) return rc;
-  rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW>, dim3((unsigned)((long)p.B * p.Hk * nkt)), NW * 64,
-                 RaDkv<T, DP, QT>::bytes(p.R), stream, p);
+  rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW>, dim3((unsigned)(p.B * p.Hk * nkt * g.ksplit)), NW * 64,
+                 RaDkv<T, DP, QT, NW>::bytes(p.R), stream, g);
   if (rc) return rc;
-  hipLaunchKernelGGL(rel_attn_dtable_kernel<T>, dim3(p.Hq), dim3(1024), 8 * (2 * (size_t)p.R + 1), (hipStream_t)stream, p,
-                     (T*)dtable, nqt);
+  const auto blocks = [&](long n) { return (n / 4 + 255) / 256; };
+  const long dq = g.qsplit > 1 ? blocks((long)p.B * p.Lq * p.Hq * p.D) : 0;
+  const long dk = g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0;
+  hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3((unsigned)(p.Hq + dq + dk)), dim3(256), 0, (hipStream_t)stream, g, (int)nkt,
+                     (int)dq);
   OCCF_LAUNCH_CHECK();
 }
 
 extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int dtype) {
   if (ra_check(geom, dtype)) return -1;
-  const long B = geom[0], Lq = geom[1], Hq = geom[3], R = geom[7];
-  return B * Hq * Lq + B * Hq * ((Lq + 127) / 128) * (2 * R + 1);
+  int qs, ks;
+  ra_bwd_plan(geom, qs, ks);
+  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, qs, ks);
+  return s.delta + s.eps + s.dq * (dtype == 1 ? 2 : 1) + s.dk * 2 + s.tab;
 }
 
 extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
@@ -447,16 +568,26 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
   if (bad) return bad;
   if (!q || !k || !v || !table || !lut || !out || !lse || !dout || !dq || !dk || !dv || !dtable || !workspace || !(scale > 0.f))
     return OCCF_EINVAL;
-  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk |
+  if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk |
         (uintptr_t)dv) & 15) != 0)
     return OCCF_EINVAL;
   if (workspace_floats < occf_rel_attn_bwd_workspace(geom, dtype)) return OCCF_EINVAL;
-  RaParams p = ra_params(geom, scale, causal);
+  RaBwd g = {};
+  g.a = ra_params(geom, scale, causal);
+  RaParams& p = g.a;
   p.q = q; p.k = k; p.v = v; p.table = table; p.lut = lut;
   p.q_lens = q_lens; p.k_lens = k_lens; p.q_start = q_start;
   p.out = out; p.dout = dout; p.lse = (float*)lse;
   p.dq = dq; p.dk = dk; p.dv = dv;
+  g.dtable = dtable;
+  ra_bwd_plan(geom, g.qsplit, g.ksplit);
+  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, g.qsplit, g.ksplit);
   p.delta = workspace;
-  p.part = workspace + (long)p.B * p.Hq * p.Lq;
-  RA_DISPATCH(dtype, p.D, ra_bwd, p, dtable, stream);
+  g.eps = p.delta + s.delta;
+  g.dq_part = g.eps + s.eps;
+  g.pk_part = g.dq_part + s.dq;
+  g.dk_part = g.pk_part + (dtype == 1 ? s.dq : 0);
+  g.dv_part = g.dk_part + s.dk;
+  g.tab_part = g.dv_part + s.dk;
+  RA_DISPATCH(dtype, p.D, ra_bwd, g, stream);
 }

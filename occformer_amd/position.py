@@ -37,8 +37,8 @@ class RelativeBuckets:
         if num_buckets > 128 or n < 2 or (bidirectional and num_buckets % 2):
             raise ValueError(f"RelativeBuckets: num_buckets {num_buckets} must be at most 128 and leave two or more a side")
         exact = n // 2
-        if not exact < max_distance <= 1024:
-            raise ValueError(f"RelativeBuckets: max_distance {max_distance} must lie in ({exact}, 1024]")
+        if not exact < max_distance <= 512:
+            raise ValueError(f"RelativeBuckets: max_distance {max_distance} must lie in ({exact}, 512]")
         self.num_buckets, self.radius, self.bidirectional = int(num_buckets), int(max_distance), bool(bidirectional)
         edges, d = [], exact
         for m in range(1, n - exact):
