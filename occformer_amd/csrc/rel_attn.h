@@ -145,23 +145,71 @@ __device__ __forceinline__ void ra_store4(ra_bf16* p, float a, float b, float c,
 
 // ---- a 4 x 4 block of a tile: 4 rows x 4 columns on their way from global memory to the LDS images
 template <class T> struct RaBlk;
-template <> struct RaBlk<float> { float4 r[4]; };
-template <> struct RaBlk<ra_bf16> { struct { uint32_t x, y; } r[4]; };
 
-// block u of a tile of `rows` x DP (u = row group * (DP / 4) + column group); rows at or behind `limit` and columns at or
-// behind D are zero
+// bounded loads (one select on a 32-bit offset instead of a branch a load: under branches every load is waited for where the
+// paths meet).  The resource starts at the tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows
+// span less than 2 GiB (ra_check)
+#ifdef OCCF_EMU
+static inline RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
+  const occf_u32x4 v = occf_bbuf_load_b128(b, off);
+  return RaU4{{v.x, v.y, v.z, v.w}};
+}
+struct ra_raw2 { uint32_t x, y; };
+static inline ra_raw2 ra_buf8(occf_bbuf b, uint32_t off) {
+  ra_raw2 v = {0u, 0u};
+  if ((uint64_t)off + 8u <= (uint64_t)b.nbytes) memcpy(&v, b.base + off, 8);
+  return v;
+}
+#else
+__device__ __forceinline__ RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
+  return __builtin_bit_cast(RaU4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+struct ra_raw2 { uint32_t x, y; };
+__device__ __forceinline__ ra_raw2 ra_buf8(occf_bbuf b, uint32_t off) {
+  return __builtin_bit_cast(ra_raw2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
+}
+#endif
+__device__ __forceinline__ occf_bbuf ra_buf(const void* p) { return occf_make_bbuf(p, 0x7FFFFFFFu); }
+template <> struct RaBlk<float> { RaU4 r[4]; };
+template <> struct RaBlk<ra_bf16> { ra_raw2 r[4]; };
+
+// block u of a tile (u = row group * (DP / 4) + column group): `tile` points at row 0, rows at or behind `rows` and columns at
+// or behind D are zero; stride in elements
 template <class T, int DP>
-__device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, const T* base, long stride, int row0, int limit, int D, int u) {
-  const int cg = u % (DP / 4), rg = u / (DP / 4);
-  const int c = cg * 4;
+__device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, const T* tile, long stride, int rows, int D, int u) {
+  const int c = (u % (DP / 4)) * 4, r0 = (u / (DP / 4)) * 4;
+  const occf_bbuf buf = ra_buf(tile);
+  const uint32_t step = (uint32_t)stride * (uint32_t)sizeof(T);
+  const uint32_t at = (uint32_t)r0 * step + (uint32_t)(c * sizeof(T));
+  const int n = c < D ? rows - r0 : 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int row = row0 + rg * 4 + i;
-    b.r[i] = {};
-    if (row < limit && c < D) {
-      typedef decltype(b.r[i]) V;
-      b.r[i] = *(const std::remove_reference_t<V>*)__builtin_assume_aligned(base + (long)row * stride + c, sizeof(T) * 4);
+    const uint32_t off = i < n ? at + i * step : OCCF_BUF_OOB;
+    if constexpr (sizeof(T) == 4) b.r[i] = ra_buf16(buf, off);
+    else b.r[i] = ra_buf8(buf, off);
+  }
+}
+
+// fragment of 8 columns from `c` of row `row` of such a tile
+template <class T>
+__device__ __forceinline__ RaFrag<RaType<T>::NT> ra_tile_frag(const T* tile, long stride, int row, int rows, int c, int D) {
+  const occf_bbuf buf = ra_buf(tile);
+  const uint32_t at = (uint32_t)row * ((uint32_t)stride * (uint32_t)sizeof(T)) + (uint32_t)(c * sizeof(T));
+  const bool ok = row < rows && c < D;
+  if constexpr (RaType<T>::NT == 1) {
+    const RaU4 x = ra_buf16(buf, ok ? at : OCCF_BUF_OOB);
+    RaFrag<1> f;
+    f.p[0] = ra_as_frag(x.x[0], x.x[1], x.x[2], x.x[3]);
+    return f;
+  } else {
+    const RaU4 x = ra_buf16(buf, ok ? at : OCCF_BUF_OOB), y = ra_buf16(buf, ok ? at + 16 : OCCF_BUF_OOB);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = occf_u2f(x.x[e]);
+      f[4 + e] = occf_u2f(y.x[e]);
     }
+    return ra_pack8<3>(f);
   }
 }
 
@@ -177,10 +225,10 @@ __device__ __forceinline__ void ra_blk_pieces(const RaBlk<float>& b, uint32_t (&
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t s[3];
-    ra_split2<3>(b.r[i].x, b.r[i].y, s);
+    ra_split2<3>(occf_u2f(b.r[i].x[0]), occf_u2f(b.r[i].x[1]), s);
 #pragma unroll
     for (int t = 0; t < 3; ++t) w[t][i][0] = s[t];
-    ra_split2<3>(b.r[i].z, b.r[i].w, s);
+    ra_split2<3>(occf_u2f(b.r[i].x[2]), occf_u2f(b.r[i].x[3]), s);
 #pragma unroll
     for (int t = 0; t < 3; ++t) w[t][i][1] = s[t];
   }
@@ -301,6 +349,22 @@ __device__ __forceinline__ f32x16 ra_splat16(float x) {
   return z;
 }
 
+// Workgroup -> (tile, head of the batch).  Equal tiles: an XCD takes whole heads one after another (their keys stay in its L2).
+// Causal ones differ in length: `t` = 0, the longest, of up to 64 heads first, so that short ones fill the gaps at the end; the
+// heads go round the XCDs, eight or a multiple of them keep each to its own.
+__device__ __forceinline__ void ra_order(const RaParams& p, unsigned bid, unsigned ntile, unsigned heads, int& t, int& bh) {
+  if (!p.causal) {
+    bid = occf_xcd_remap(bid, gridDim.x);
+    t = (int)(bid % ntile);
+    bh = (int)(bid / ntile);
+    return;
+  }
+  const unsigned chunk = bid / (64 * ntile), in = bid - chunk * 64 * ntile;
+  const unsigned n = heads - chunk * 64 < 64 ? heads - chunk * 64 : 64;
+  t = (int)(in / n);
+  bh = (int)(chunk * 64 + in % n);
+}
+
 // rows of sequence b that count: queries [0, nq), keys [0, nk), position of query 0
 __device__ __forceinline__ void ra_lengths(const RaParams& p, int b, int& nq, int& nk, int& start) {
   nq = p.q_lens ? occf_clampi(p.q_lens[b], p.Lq) : p.Lq;
@@ -322,7 +386,9 @@ static int ra_check(const int64_t* g, int dtype) {
   if (Lq * (Hq / Hk) >= (1L << 30) || B * Hk * ((Lq * (Hq / Hk) + 31) / 32) * 64 >= 2147483647L) return OCCF_ESHAPE;
   const long per16 = dtype == 0 ? 4 : 8;
   for (int s = 8; s < 17; ++s)
-    if (g[s] % per16) return OCCF_ESHAPE;
+    if (g[s] < 0 || g[s] % per16) return OCCF_ESHAPE;
+  for (int s = 9; s < 17; s += 3)
+    if (g[s] >= (1L << 22)) return OCCF_ESHAPE;          // 64 rows within 2 GiB
   return 0;
 }
 

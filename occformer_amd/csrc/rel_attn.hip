@@ -28,13 +28,10 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
   const int nqt = (p.Lq + 127) / 128;
-  unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  // causal rows differ in length: every other head walks them the other way, so that the workgroups that one compute unit
-  // holds (a fixed step apart) add up to the same work
-  const int back = (int)(bid % nqt);
-  bid /= nqt;
-  const int qt = bid & 1 ? back : nqt - 1 - back;
-  const int h = (int)(bid % p.Hq), b = (int)(bid / p.Hq);
+  int qt, bh;
+  ra_order(p, blockIdx.x, nqt, p.B * p.Hq, qt, bh);
+  qt = nqt - 1 - qt;                                     // the last queries see the most keys
+  const int h = bh % p.Hq, b = bh / p.Hq;
   const int hk = h / (p.Hq / p.Hk);
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
@@ -72,8 +69,8 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % 256 && tid + n * 256 >= NB) break;
-      ra_load_blk<T, DP>(rk[n], kb, p.ksl, 0, kend, p.D, tid + n * 256);
-      ra_load_blk<T, DP>(rv[n], vb, p.vsl, 0, kend, p.D, tid + n * 256);
+      ra_load_blk<T, DP>(rk[n], kb, p.ksl, kend, p.D, tid + n * 256);
+      ra_load_blk<T, DP>(rv[n], vb, p.vsl, kend, p.D, tid + n * 256);
     }
   }
   for (int kt = 0; kt < ntile; ++kt) {
@@ -93,8 +90,8 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 #pragma unroll
       for (int n = 0; n < NU; ++n) {
         if (NB % 256 && tid + n * 256 >= NB) break;
-        ra_load_blk<T, DP>(rk[n], kb, p.ksl, k0 + KT, kend, p.D, tid + n * 256);
-        ra_load_blk<T, DP>(rv[n], vb, p.vsl, k0 + KT, kend, p.D, tid + n * 256);
+        ra_load_blk<T, DP>(rk[n], kb + (k0 + KT) * p.ksl, p.ksl, kend - k0 - KT, p.D, tid + n * 256);
+        ra_load_blk<T, DP>(rv[n], vb + (k0 + KT) * p.vsl, p.vsl, kend - k0 - KT, p.D, tid + n * 256);
       }
     }
     if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
@@ -239,18 +236,13 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 32 ? 2 : 1) r
 
   RaFrag<NT> kf[KS];
   RaBlk<T> rv[NV];
-  int j0 = first + wave * 32;
+  int j0 = first + occf_wave_uniform(wave) * 32;
   auto load = [&](int at) {
-    const bool ok = at + li < lim;
-    const T* krow = kb + (long)(ok ? at + li : 0) * p.ksl;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = ks * 16 + lk * 8;
-      kf[ks] = ra_row_frag<T>(krow + (d < p.D ? d : 0), ok && d < p.D);
-    }
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = ra_tile_frag<T>(kb + at * p.ksl, p.ksl, li, lim - at, ks * 16 + lk * 8, p.D);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
-      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T, DP>(rv[n], vb, p.vsl, at, lim, p.D, lane + n * 64);
+      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T, DP>(rv[n], vb + at * p.vsl, p.vsl, lim - at, p.D, lane + n * 64);
   };
   if (j0 < lim) load(j0);
   for (; j0 < lim; j0 += RA_WAVES * 32) {

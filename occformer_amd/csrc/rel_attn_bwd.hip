@@ -20,7 +20,12 @@
 #include "rel_attn.h"
 #include "../../include/occformer_hip.h"
 
-#define RA_DLD 33               // row of the 32 x 32 tile whose diagonals are summed
+// Half a 32 x 32 tile whose diagonals are summed: rows of 72 floats of which the last 40 stay zero, as do 32 before the first,
+// so that a lane's walk down its diagonal needs no test (16 reads at constant offsets).  A whole tile would leave room for one
+// workgroup a compute unit instead of two (523 instead of 409 us at 2 x 4096 causal rows, 16 heads of 64).
+#define RA_DLD 72
+#define RA_DFRONT 32
+#define RA_DTILE (RA_DFRONT + 16 * RA_DLD)
 
 struct RaBwd {
   RaParams a;
@@ -50,13 +55,12 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
 
   const int nqt = (p.Lq + QW - 1) / QW;
-  unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  const int back = (int)(bid % nqt);
-  bid /= nqt;
-  const int qt = bid & 1 ? back : nqt - 1 - back;        // (see rel_attn_fwd_kernel)
-  const int split = (int)(bid % g.qsplit);
-  bid /= g.qsplit;
-  const int h = (int)(bid % p.Hq), b = (int)(bid / p.Hq);
+  int qt, bh;
+  ra_order(p, blockIdx.x, nqt, p.B * p.Hq * g.qsplit, qt, bh);
+  qt = nqt - 1 - qt;
+  const int split = bh % g.qsplit;
+  bh /= g.qsplit;
+  const int h = bh % p.Hq, b = bh / p.Hq;
   const int hk = h / (p.Hq / p.Hk);
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
@@ -111,8 +115,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T, DP>(rk[n], kb, p.ksl, k0, kend, p.D, tid + n * TH);
-      ra_load_blk<T, DP>(rv[n], vb, p.vsl, k0, kend, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(rk[n], kb + k0 * p.ksl, p.ksl, kend - k0, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(rv[n], vb + k0 * p.vsl, p.vsl, kend - k0, p.D, tid + n * TH);
     }
   };
   if (t0 < t1) load(t0 * KT);
@@ -198,7 +202,7 @@ struct RaDkv {
   static constexpr int NT = RaType<T>::NT;
   static constexpr int images = 2 * NT * (RaRow<DP>::bytes(QT) + RaTrans<QT>::bytes(DP));
   static size_t bytes(int R) {
-    return images + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + 2 * QT + NW * 32 * RA_DLD);
+    return images + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + 2 * QT + NW * RA_DTILE);
   }
 };
 
@@ -215,21 +219,20 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   float* s_lse = (float*)(img_ot + NT * RaTrans<QT>::bytes(DP));       // first values of the accumulators' rows
   float* s_delta = s_lse + QT;
   float* tiles = s_delta + QT;
-  float* lut = tiles + NW * 32 * RA_DLD;
+  float* lut = tiles + NW * RA_DTILE;
   const int nl = 2 * p.R + 1 + 2 * RA_PAD;
   float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
   float* dsum = sums + wave * nl;
-  float* tile = tiles + wave * 32 * RA_DLD;
+  float* tile = tiles + wave * RA_DTILE + RA_DFRONT;
+  for (int t = tid; t < NW * RA_DTILE; t += TH) tiles[t] = 0.f;
 
   const int nkt = (p.Lk + KW - 1) / KW, G = p.Hq / p.Hk;
-  unsigned bid = occf_xcd_remap(blockIdx.x, gridDim.x);
-  const int back = (int)(bid % nkt);
-  bid /= nkt;
-  const int kt = bid & 1 ? nkt - 1 - back : back;
-  const int split = (int)(bid % g.ksplit);
-  bid /= g.ksplit;
-  const int hk = (int)(bid % p.Hk), b = (int)(bid / p.Hk);
+  int kt, bh;
+  ra_order(p, blockIdx.x, nkt, p.B * p.Hk * g.ksplit, kt, bh);         // the first keys are seen by the most queries
+  const int split = bh % g.ksplit;
+  bh /= g.ksplit;
+  const int hk = bh % p.Hk, b = bh / p.Hk;
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
 
@@ -280,8 +283,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T, DP>(rq[n], qb, p.qsl, r0, nq, p.D, tid + n * TH);
-      ra_load_blk<T, DP>(ro[n], ob, (long)p.Hq * p.D, r0, nq, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(rq[n], qb + r0 * p.qsl, p.qsl, nq - r0, p.D, tid + n * TH);
+      ra_load_blk<T, DP>(ro[n], ob + (long)r0 * p.Hq * p.D, (long)p.Hq * p.D, nq - r0, p.D, tid + n * TH);
     }
     if (tid < QT) {
       const int i = r0 + tid;
@@ -349,17 +352,18 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       }
       if (near) {
         // sums along the diagonals: lane e adds the pairs at distance rel0 + e - 31 (63 of them), in LDS of the wave's own
-        RA_WAVE_SYNC();
+        float y[2] = {0.f, 0.f};
+        const float* dg = tile + lane - 31;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * RA_DLD + li] = ds[r];
-        RA_WAVE_SYNC();
-        float x = 0.f;
-#pragma unroll 8
-        for (int q = 0; q < 32; ++q) {
-          const int col = q + lane - 31;
-          const float y = tile[q * RA_DLD + occf_clampi(col, 31)];
-          x += col >= 0 && col < 32 ? y : 0.f;
+        for (int hv = 0; hv < 2; ++hv) {
+          RA_WAVE_SYNC();
+#pragma unroll
+          for (int r = 0; r < 8; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * RA_DLD + li] = ds[8 * hv + r];
+          RA_WAVE_SYNC();
+#pragma unroll
+          for (int q = 0; q < 16; ++q) y[q & 1] += dg[q * (RA_DLD + 1) + 16 * hv];
         }
+        const float x = y[0] + y[1];
         if (lane < 63) dsum[rel0 + lane - 31 + p.R + RA_PAD] += x;
       } else {
         float x = 0.f;
