@@ -13,14 +13,17 @@
 #include "occf_common.h"
 
 #define RA_LOG2E 1.44269504088896340736f
-#define RA_WAVES 4
 #define RA_PAD 64               // bias columns kept beyond either end of the clamped distances
 
 #ifdef OCCF_EMU
+#define ra_mfma16(a, b, c) emu_mfma_f32_16x16x32_bf16(a, b, c)
 #define RA_WAVE_SYNC() hipemu::wave_sync()
 static inline float ra_exp2(float x) { return exp2f(x); }
 static inline float ra_log2(float x) { return log2f(x); }
 #else
+typedef __bf16 ra_bf16x8 __attribute__((ext_vector_type(8)));
+#define ra_mfma16(a, b, c) \
+  __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ra_bf16x8, a), __builtin_bit_cast(ra_bf16x8, b), c, 0, 0, 0)
 // a wave's own LDS writes become visible to its other lanes (LDS operations of one wave complete in order)
 #define RA_WAVE_SYNC()                                    \
   do {                                                    \
@@ -47,7 +50,7 @@ struct RaParams {
   void *o, *dq, *dk, *dv;
   float *lse, *delta, *part;
   long qsb, qsl, qsh, ksb, ksl, ksh, vsb, vsl, vsh;     // element strides: batch, row, head
-  int B, Lq, Lk, Hq, Hk, D, nb, R, causal, nsplit, chunk;
+  int B, Lq, Lk, Hq, Hk, D, nb, R, causal, nsplit, chunk, units, by_length;
   float scale, c;                                          // c = scale * log2(e)
 };
 
@@ -143,6 +146,21 @@ __device__ __forceinline__ void ra_store4(ra_bf16* p, float a, float b, float c,
   *(U2*)__builtin_assume_aligned(p, 8) = U2{occf_bf16_pack2(a, b), occf_bf16_pack2(c, d)};
 }
 
+// LDS images of a tile of ROWS x DP, one per piece.
+//   row image:   [ROWS][DP], 16 bytes of padding a row: the 16-lane groups of a b128 read hit 16 different bank quads
+//   trans image: [DP][ROWS], 4-row groups in operand order, 16 bytes of padding, the 16-byte slots of a row exchanged by
+//                (column >> 4) & 3 so that the 16 column groups of a store do not meet on one bank quad
+template <int DP> struct RaRow {
+  static constexpr int LD = DP * 2 + 16;
+  static constexpr int bytes(int rows) { return rows * LD; }
+};
+template <int ROWS> struct RaTrans {
+  static constexpr int LD = ROWS * 2 + 16;
+  static constexpr int bytes(int dp) { return dp * LD; }
+};
+
+typedef uint32_t ra_u2 __attribute__((ext_vector_type(2)));
+
 // ---- a 4 x 4 block of a tile: 4 rows x 4 columns on their way from global memory to the LDS images
 template <class T> struct RaBlk;
 
@@ -190,27 +208,26 @@ __device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, const T* tile, long str
   }
 }
 
-// fragment of 8 columns from `c` of row `row` of such a tile
+// 8 columns from `c` of row `row` of such a tile, as loaded and as a fragment
+template <class T> struct RaRaw { RaU4 x[sizeof(T) / 2]; };
 template <class T>
-__device__ __forceinline__ RaFrag<RaType<T>::NT> ra_tile_frag(const T* tile, long stride, int row, int rows, int c, int D) {
+__device__ __forceinline__ void ra_load_raw(RaRaw<T>& f, const T* tile, long stride, int row, int rows, int c, int D) {
   const occf_bbuf buf = ra_buf(tile);
   const uint32_t at = (uint32_t)row * ((uint32_t)stride * (uint32_t)sizeof(T)) + (uint32_t)(c * sizeof(T));
-  const bool ok = row < rows && c < D;
-  if constexpr (RaType<T>::NT == 1) {
-    const RaU4 x = ra_buf16(buf, ok ? at : OCCF_BUF_OOB);
-    RaFrag<1> f;
-    f.p[0] = ra_as_frag(x.x[0], x.x[1], x.x[2], x.x[3]);
-    return f;
-  } else {
-    const RaU4 x = ra_buf16(buf, ok ? at : OCCF_BUF_OOB), y = ra_buf16(buf, ok ? at + 16 : OCCF_BUF_OOB);
-    float f[8];
+  const uint32_t off = row < rows && c < D ? at : OCCF_BUF_OOB;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[e] = occf_u2f(x.x[e]);
-      f[4 + e] = occf_u2f(y.x[e]);
-    }
-    return ra_pack8<3>(f);
-  }
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) f.x[e] = ra_buf16(buf, off + 16u * e);
+}
+__device__ __forceinline__ RaFrag<1> ra_raw_frag(const RaRaw<ra_bf16>& w) {
+  RaFrag<1> f;
+  f.p[0] = ra_as_frag(w.x[0].x[0], w.x[0].x[1], w.x[0].x[2], w.x[0].x[3]);
+  return f;
+}
+__device__ __forceinline__ RaFrag<3> ra_raw_frag(const RaRaw<float>& w) {
+  float f[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = occf_u2f(w.x[e >> 2].x[e & 3]);
+  return ra_pack8<3>(f);
 }
 
 // block -> packed pieces, w[piece][row][pair of columns]
@@ -234,20 +251,6 @@ __device__ __forceinline__ void ra_blk_pieces(const RaBlk<float>& b, uint32_t (&
   }
 }
 
-// LDS images of a tile of ROWS x DP, one per piece.
-//   row image:   [ROWS][DP], 16 bytes of padding a row: the 16-lane groups of a b128 read hit 16 different bank quads
-//   trans image: [DP][ROWS], 4-row groups in operand order, 16 bytes of padding, the 16-byte slots of a row exchanged by
-//                (column >> 4) & 3 so that the 16 column groups of a store do not meet on one bank quad
-template <int DP> struct RaRow {
-  static constexpr int LD = DP * 2 + 16;
-  static constexpr int bytes(int rows) { return rows * LD; }
-};
-template <int ROWS> struct RaTrans {
-  static constexpr int LD = ROWS * 2 + 16;
-  static constexpr int bytes(int dp) { return dp * LD; }
-};
-
-typedef uint32_t ra_u2 __attribute__((ext_vector_type(2)));
 
 template <int NT, int DP, int ROWS>
 __device__ __forceinline__ void ra_store_row(char* img, const uint32_t (&w)[NT][4][2], int u) {
@@ -261,12 +264,12 @@ __device__ __forceinline__ void ra_store_row(char* img, const uint32_t (&w)[NT][
     }
 }
 
-template <int NT, int DP, int ROWS>
+template <int NT, int DP, int ROWS, int COLS = 32>
 __device__ __forceinline__ void ra_store_trans(char* img, const uint32_t (&w)[NT][4][2], int u) {
   const int c = (u % (DP / 4)) * 4, rg = u / (DP / 4);
   // row group g of a 16-row step holds k values lk = g & 1, e = 4 (g >> 1) ..: 8-byte slot 2 lk + (g >> 1)
-  const int g = rg & 3, slot = (rg >> 2) * 2 + (g & 1);
-  const int off = ((slot ^ ((c >> 4) & 3)) * 16) + (g >> 1) * 8;
+  const int g = rg & 3, slot = COLS == 16 ? g : (rg >> 2) * 2 + (g & 1), half = COLS == 16 ? rg >> 2 : g >> 1;
+  const int off = ((slot ^ ((c >> 4) & 3)) * 16) + half * 8;
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -294,6 +297,16 @@ __device__ __forceinline__ RaFrag<NT> ra_read_row(const char* img, int row0, int
     f.p[t] = *(const bf16x8*)(img + t * RaRow<DP>::bytes(ROWS) + (row0 + li) * RaRow<DP>::LD + ks * 32 + lk * 16);
   return f;
 }
+// A operand of the 16-column form: 16 columns of the tile from c0, its 32 rows; g = lane >> 4
+template <int NT, int DP>
+__device__ __forceinline__ RaFrag<NT> ra_read_trans16(const char* img, int c0, int li, int g) {
+  RaFrag<NT> f;
+  const int d = c0 + li;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+    f.p[t] = *(const bf16x8*)(img + t * RaTrans<32>::bytes(DP) + d * RaTrans<32>::LD + ((g ^ ((d >> 4) & 3)) * 16));
+  return f;
+}
 // A operand: 32 columns of the tile from c0, k step ks of 16 tile rows
 template <int NT, int DP, int ROWS>
 __device__ __forceinline__ RaFrag<NT> ra_read_trans(const char* img, int c0, int ks, int li, int lk) {
@@ -304,6 +317,21 @@ __device__ __forceinline__ RaFrag<NT> ra_read_trans(const char* img, int c0, int
     f.p[t] = *(const bf16x8*)(img + t * RaTrans<ROWS>::bytes(DP) + d * RaTrans<ROWS>::LD +
                               (((ks * 2 + lk) ^ ((d >> 4) & 3)) * 16));
   return f;
+}
+
+// ---- the same chain on 16 columns (v_mfma_f32_16x16x32_bf16): a lane holds column lane & 15 and, of 32 tile rows in two
+// accumulators, rows 16 (e >> 2) + 4 (lane >> 4) + (e & 3), e = 0..7, which are one B operand of 32 k-values; the transposed
+// image keeps row group g = row >> 2 at 16-byte slot g & 3, half g >> 2.
+template <int NT>
+__device__ __forceinline__ f32x4 ra_mm16(const RaFrag<NT>& a, const RaFrag<NT>& b, f32x4 c) {
+  if constexpr (NT == 3) {
+    c = ra_mfma16(a.p[2], b.p[0], c);
+    c = ra_mfma16(a.p[0], b.p[2], c);
+    c = ra_mfma16(a.p[1], b.p[1], c);
+    c = ra_mfma16(a.p[1], b.p[0], c);
+    c = ra_mfma16(a.p[0], b.p[1], c);
+  }
+  return ra_mfma16(a.p[0], b.p[0], c);
 }
 
 // a table entry in the base-2 domain; entries at or under -1e30 take their bucket out
@@ -349,12 +377,13 @@ __device__ __forceinline__ f32x16 ra_splat16(float x) {
   return z;
 }
 
-// Workgroup -> (tile, head of the batch).  Equal tiles: an XCD takes whole heads one after another (their keys stay in its L2).
-// Causal ones differ in length: `t` = 0, the longest, of up to 64 heads first, so that short ones fill the gaps at the end; the
-// heads go round the XCDs, eight or a multiple of them keep each to its own.
+// Workgroup -> (tile, head of the batch).  Tiles of a head, and heads from tile to tile, go round the XCDs (workgroup n runs on
+// XCD n mod 8), so that sequences of differing length spread over all of them; a head's workgroups walk its keys side by side and
+// find them in their L2.  (Whole heads to an XCD leave some with the short sequences: 92 ... 157 instead of 67 us at 4 x 2500 fp32
+// tokens of 0 ... 2500.)  Causal tiles differ in length: of 64 heads at a time the longest (`t` = 0) go first, so that short ones
+// fill the gaps at the end; heads keep to their XCDs there unless a sequence has fewer than eight of them.
 __device__ __forceinline__ void ra_order(const RaParams& p, unsigned bid, unsigned ntile, unsigned heads, int& t, int& bh) {
   if (!p.causal) {
-    bid = occf_xcd_remap(bid, gridDim.x);
     t = (int)(bid % ntile);
     bh = (int)(bid / ntile);
     return;
@@ -362,7 +391,7 @@ __device__ __forceinline__ void ra_order(const RaParams& p, unsigned bid, unsign
   const unsigned chunk = bid / (64 * ntile), in = bid - chunk * 64 * ntile;
   const unsigned n = heads - chunk * 64 < 64 ? heads - chunk * 64 : 64;
   t = (int)(in / n);
-  bh = (int)(chunk * 64 + in % n);
+  bh = (int)(chunk * 64 + (in + (heads < 8u * p.B ? t : 0)) % n);
 }
 
 // rows of sequence b that count: queries [0, nq), keys [0, nk), position of query 0

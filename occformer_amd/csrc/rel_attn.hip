@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
   }
   if (i >= p.Lq) return;
   l += __shfl_xor(l, 32);
-  const bool some = l > 0.f && i < nq;                   // rows behind the last query went along with their tile
+  const bool some = l != 0.f && i < nq;                   // rows behind the last query went along with their tile
   const float inv = some ? 1.0f / l : 0.f;
   if (!some) {
 #pragma unroll
@@ -168,121 +168,218 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Few queries: the rows of one key head (query i of its G query heads, row = i G + g) in groups of 32 share every key that
-// is read.  The keys are split over workgroups and, tile by tile, over a workgroup's four waves; a wave reads its
-// key rows straight into operand registers and turns its value rows round in LDS of its own, so that no wave waits for
-// another before the join at the end.  part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
-template <class T, int DP>
+// Parts by the sequences' own lengths.  Equal parts of the longest leave the card half empty when lengths differ (16 sequences
+// of 0 ... 8192 keys: 72 us at 4 parts each), and many small ones cost about 10 us a workgroup to begin and end.  So the keys of
+// all sequences are counted, a part is their share of nsplit B parts (in steps of 128), and sequence b gets ceil(len_b / part)
+// consecutive units of the B nsplit + B there are at most.  `unit` >= 0: which sequence and part it is (false: none);
+// else `seq`: its first unit (in `split`) and their number n.  One wave's lanes hold 64 sequences at a time.
+__device__ __forceinline__ bool ra_unit(const RaParams& p, int unit, int seq, int& b, int& split, int& n, int& chunk) {
+  const int lane = threadIdx.x & 63;
+  long total = 0;
+  for (int s0 = 0; s0 < p.B; s0 += 64) {
+    int x = s0 + lane < p.B ? occf_clampi(p.k_lens[s0 + lane], p.Lk) : 0;
+    long y = x;
+#pragma unroll
+    for (int mm = 32; mm > 0; mm >>= 1) y += __shfl_xor(y, mm);
+    total += y;
+  }
+  const long parts = (long)p.B * p.nsplit;
+  chunk = (int)(((total + parts - 1) / parts + 127) / 128 * 128);
+  chunk = chunk < 128 ? 128 : chunk;
+  int before = 0;
+  for (int s0 = 0; s0 < p.B; s0 += 64) {
+    const int x = s0 + lane < p.B ? occf_clampi(p.k_lens[s0 + lane], p.Lk) : 0;
+    const int c = (x + chunk - 1) / chunk;
+    int sum = c;                                         // units up to and with this lane's sequence
+#pragma unroll
+    for (int mm = 1; mm < 64; mm <<= 1) {
+      const int y = __shfl_up(sum, mm);
+      if (lane >= mm) sum += y;
+    }
+    sum += before;
+    if (unit >= 0) {
+      const int at = __popcll(__ballot(sum <= unit));
+      if (at < 64 && s0 + at < p.B) {
+        b = s0 + at;
+        n = __shfl(c, at);
+        split = unit - (__shfl(sum, at) - n);
+        return true;
+      }
+    } else if (seq < s0 + 64) {
+      n = __shfl(c, seq - s0);
+      split = __shfl(sum, seq - s0) - n;
+      return true;
+    }
+    before = __shfl(sum, 63);
+  }
+  return false;
+}
+
+// Few queries: the rows of one key head (query i of its G query heads, row = i G + g) in groups of RW = 32, or 16 where there are
+// no more, share every key that is read.  The keys are split over workgroups and, tile by tile, over a workgroup's four waves;
+// a wave reads its key rows straight into operand registers and turns its value rows round in LDS of its own, so that no wave
+// waits for another before the join at the end.  (Keys through LDS, in whole rows of the cache line, took 99 instead of 67 us for
+// 4 x 2500 fp32 queries and as long for single ones.)  Bound by the stream of keys and values: 16 rows take half the
+// accumulators, products and exponentials of 32, which leaves room for a second tile in flight.
+// part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
+template <class T, int DP, int RW>
 struct RaFew {
-  static constexpr int NT = RaType<T>::NT, VT = NT * RaTrans<32>::bytes(DP);
-  static constexpr int join = 32 * (DP + 4) * 4;         // [32 rows][DP + 4] floats of one wave
+  static constexpr int NT = RaType<T>::NT, NW = 4, VT = NT * RaTrans<32>::bytes(DP);
+  static constexpr int join = RW * (DP + 4) * 4;         // [RW rows][DP + 4] floats of one wave
   static constexpr int wave = VT > join ? VT : join;
+  static size_t bytes(int nb, int R) { return NW * wave + 4 * ((size_t)nb * RW + 2 * R + 1 + (2 * NW + 2) * RW); }
 };
 
-template <class T, int DP>
-__global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 32 ? 2 : 1) rel_attn_few_kernel(RaParams p) {
-  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
-  constexpr int NB = 2 * DP, NV = (NB + 63) / 64;                        // 4 x 4 blocks of 32 value rows, and a lane's share
+template <class T, int DP, int RW>
+__global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 1 || DP <= 32 ? 2 : 1)
+    rel_attn_few_kernel(RaParams p) {
+  constexpr int NT = RaType<T>::NT, NW = RaFew<T, DP, RW>::NW, TH = NW * 64;
+  constexpr int NE = RW / 2;                             // scores of a 32-key tile a lane holds
+  constexpr int QS = DP / (RW == 32 ? 16 : 32);          // k steps of Q K^T
+  constexpr int KR = DP / 16;                            // key fragments: [k step] or [16-key half][k step]
+  constexpr int DT = DP / RW;                            // column tiles of the output
+  constexpr int NB = 2 * DP, NV = (NB + 63) / 64;        // 4 x 4 blocks of 32 value rows, and a lane's share
+  typedef typename std::conditional<RW == 32, f32x16, f32x4>::type Acc;
   OCCF_DYN_SMEM(smem);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
-  char* img_v = smem + wave * RaFew<T, DP>::wave;
-  float* tab = (float*)(smem + RA_WAVES * RaFew<T, DP>::wave);          // [nb][32] bias of row li
-  int* lut = (int*)(tab + p.nb * 32);                                   // [2 R + 1] bucket of a distance
-  float* stat = (float*)(lut + 2 * p.R + 1);                            // [2 RA_WAVES + 2][32]
+  const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & (RW - 1), lg = lane / RW;
+  char* img_v = smem + wave * RaFew<T, DP, RW>::wave;
+  float* tab = (float*)(smem + NW * RaFew<T, DP, RW>::wave);            // [nb][RW] bias of row li
+  int* lut = (int*)(tab + p.nb * RW);                                   // [2 R + 1] bucket of a distance
+  float* stat = (float*)(lut + 2 * p.R + 1);                            // [2 NW + 2][RW]
+  const auto key_of = [&](int e) { return RW == 32 ? (e & 3) + 8 * (e >> 2) + 4 * lg : 16 * (e >> 2) + 4 * lg + (e & 3); };
 
-  const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
-  const unsigned split = blockIdx.x % p.nsplit, group = blockIdx.x / p.nsplit;
-  unsigned bid = group;
-  const int rt = (int)(bid % nrt);
-  bid /= nrt;
-  const int hk = (int)(bid % p.Hk), b = (int)(bid / p.Hk);
+  const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + RW - 1) / RW;
+  int rt, bh, b, split, chunk = p.chunk;
+  ra_order(p, blockIdx.x, nrt, p.units * p.Hk, rt, bh);
+  rt = nrt - 1 - rt;                                     // the last queries see the most keys
+  // split walks: units go round the XCDs and every XCD sees all heads (rows of one head are a fixed 256 bytes of a wider row, and
+  // an L2's 16 channels are 256 bytes wide: one head alone would keep two of them busy)
+  int hk, unit;
+  if (p.part) {
+    hk = bh / p.units;
+    unit = bh - hk * p.units;
+  } else {
+    unit = bh / p.Hk;
+    hk = bh - unit * p.Hk;
+  }
+  if (p.by_length) {
+    int n;
+    if (!ra_unit(p, unit, -1, b, split, n, chunk)) return;
+    b = occf_wave_uniform(b);                            // (came by shuffles: addresses of scalar resources)
+    split = occf_wave_uniform(split);
+    chunk = occf_wave_uniform(chunk);
+  } else {
+    b = unit / p.nsplit;
+    split = unit - b * p.nsplit;
+  }
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
-  const int row = rt * 32 + li;
+  const int row = rt * RW + li;
   const int i = row / G, h = hk * G + row % G;
   const bool live = row < rows && i < nq;
   const int pi = start + i;
-  const int i_first = (rt * 32) / G, i_last = (rt * 32 + 31 < rows ? rt * 32 + 31 : rows - 1) / G;
-
-  for (int t = tid; t < p.nb * 32; t += 256) {
-    const int r = rt * 32 + (t & 31);
-    tab[t] = r < rows ? ra_bias(ra_to_float(((const T*)p.table)[(long)(t >> 5) * p.Hq + hk * G + r % G])) : 0.f;
-  }
-  for (int t = tid; t < 2 * p.R + 1; t += 256) lut[t] = occf_clampi(p.lut[t], p.nb - 1) * 32;
-
-  const T* qrow = (const T*)p.q + (long)b * p.qsb + (long)(live ? i : 0) * p.qsl + (long)(live ? h : 0) * p.qsh;
-  RaFrag<NT> qf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int d = ks * 16 + lk * 8;
-    qf[ks] = ra_row_frag<T>(qrow + (d < p.D ? d : 0), live && d < p.D);
-  }
+  const int i_first = (rt * RW) / G, i_last = (rt * RW + RW - 1 < rows ? rt * RW + RW - 1 : rows - 1) / G;
   int kend = nk;
   if (p.causal) {
     const int last = start + (i_last < nq ? i_last : nq - 1) + 1;
     kend = last < kend ? (last > 0 ? last : 0) : kend;
   }
   if (i_first >= nq) kend = 0;
-  const int first = split * p.chunk;
-  const int lim = first + p.chunk < kend ? first + p.chunk : kend;
+  const int first = split * chunk;
+  const int lim = first + chunk < kend ? first + chunk : kend;
   const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
   const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
-  __syncthreads();
 
-  f32x16 acc[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
-  float m = -INFINITY, mref = 0.f, l = 0.f;
-
-  RaFrag<NT> kf[KS];
+  // the first tile is on its way before the tables are made
+  RaRaw<T> rk[KR];
   RaBlk<T> rv[NV];
-  int j0 = first + occf_wave_uniform(wave) * 32;
+  int j0 = first + wave * 32;
   auto load = [&](int at) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) kf[ks] = ra_tile_frag<T>(kb + at * p.ksl, p.ksl, li, lim - at, ks * 16 + lk * 8, p.D);
+    for (int n = 0; n < KR; ++n) {
+      const int key = RW == 32 ? li : (n / QS) * 16 + li, c = RW == 32 ? n * 16 + lg * 8 : (n % QS) * 32 + lg * 8;
+      ra_load_raw<T>(rk[n], kb + at * p.ksl, p.ksl, key, lim - at, c, p.D);
+    }
 #pragma unroll
     for (int n = 0; n < NV; ++n)
       if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T, DP>(rv[n], vb + at * p.vsl, p.vsl, lim - at, p.D, lane + n * 64);
   };
   if (j0 < lim) load(j0);
-  for (; j0 < lim; j0 += RA_WAVES * 32) {
-    f32x16 s = ra_zero16();
+
+  const T* qrow = (const T*)p.q + (long)b * p.qsb + (long)(live ? i : 0) * p.qsl + (long)(live ? h : 0) * p.qsh;
+  RaFrag<NT> qf[QS];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = ra_mm<NT>(kf[ks], qf[ks], s);
+  for (int ks = 0; ks < QS; ++ks) {
+    const int d = (ks * (64 / RW) + lg) * 8;
+    qf[ks] = ra_row_frag<T>(qrow + (d < p.D ? d : 0), live && d < p.D);
+  }
+  if (first < lim) {
+    for (int t = tid; t < p.nb * RW; t += TH) {
+      const int r = rt * RW + t % RW;
+      tab[t] = r < rows ? ra_bias(ra_to_float(((const T*)p.table)[(long)(t / RW) * p.Hq + hk * G + r % G])) : 0.f;
+    }
+    for (int t = tid; t < 2 * p.R + 1; t += TH) lut[t] = occf_clampi(p.lut[t], p.nb - 1) * RW;
+  }
+  __syncthreads();
+
+  Acc acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < RW * RW / 64; ++r) acc[dt][r] = 0.f;
+  float m = -INFINITY, mref = 0.f, l = 0.f;
+
+  for (; j0 < lim; j0 += NW * 32) {
     RA_WAVE_SYNC();
 #pragma unroll
     for (int n = 0; n < NV; ++n)
       if (NB % 64 == 0 || lane + n * 64 < NB) {
         uint32_t w[NT][4][2];
         ra_blk_pieces(rv[n], w);
-        ra_store_trans<NT, DP, 32>(img_v, w, lane + n * 64);
+        ra_store_trans<NT, DP, 32, RW>(img_v, w, lane + n * 64);
       }
     RA_WAVE_SYNC();
-    if (j0 + RA_WAVES * 32 < lim) load(j0 + RA_WAVES * 32);
+    float s[NE];
+    if constexpr (RW == 32) {
+      f32x16 x = ra_zero16();
+#pragma unroll
+      for (int ks = 0; ks < QS; ++ks) x = ra_mm<NT>(ra_raw_frag(rk[ks]), qf[ks], x);
+#pragma unroll
+      for (int e = 0; e < NE; ++e) s[e] = x[e];
+    } else {
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < QS; ++ks) x = ra_mm16<NT>(ra_raw_frag(rk[hf * QS + ks]), qf[ks], x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[hf * 4 + e] = x[e];
+      }
+    }
+    if (j0 + NW * 32 < lim) load(j0 + NW * 32);
 
     const int lo = j0 - (start + i_last), hi = j0 + 31 - (start + i_first);        // distances of the tile
     float mx = -INFINITY;
     if (hi <= -p.R || lo >= p.R) {
       const float far = tab[lut[hi <= -p.R ? 0 : 2 * p.R] + li];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], p.c, far);
+      for (int e = 0; e < NE; ++e) s[e] = fmaf(s[e], p.c, far);
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int rel = j0 + 4 * lk + (r & 3) + 8 * (r >> 2) - pi;
-        s[r] = fmaf(s[r], p.c, tab[lut[occf_clampi(rel + p.R, 2 * p.R)] + li]);
-      }
+      for (int e = 0; e < NE; ++e)
+        s[e] = fmaf(s[e], p.c, tab[lut[occf_clampi(j0 + key_of(e) - pi + p.R, 2 * p.R)] + li]);
     }
     if (j0 + 32 > lim || (p.causal && j0 + 31 > start + i_first)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int j = j0 + 4 * lk + (r & 3) + 8 * (r >> 2);
-        if (j >= lim || (p.causal && j > pi)) s[r] = -INFINITY;
+      for (int e = 0; e < NE; ++e) {
+        const int j = j0 + key_of(e);
+        s[e] = j >= lim || (p.causal && j > pi) ? -INFINITY : s[e];
       }
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    for (int e = 0; e < NE; ++e) mx = fmaxf(mx, s[e]);
+#pragma unroll
+    for (int mm = RW; mm < 64; mm <<= 1) mx = fmaxf(mx, __shfl_xor(mx, mm));
     if (__ballot(mx > m + RA_EXCEED)) {
       const float mn = fmaxf(m, mx);
       const float a = ra_exp2(m - (mn == -INFINITY ? 0.f : mn));
@@ -292,103 +389,112 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 32 ? 2 : 1) r
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
+        for (int r = 0; r < RW * RW / 64; ++r) acc[dt][r] *= a;
     }
-    float pv[16];
+    float pv[NE];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      pv[r] = ra_exp2(s[r] - mref);
-      l += pv[r];
+    for (int e = 0; e < NE; ++e) {
+      pv[e] = ra_exp2(s[e] - mref);
+      l += pv[e];
     }
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
+    for (int s2 = 0; s2 < NE / 8; ++s2) {
       const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-        acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, li, lk), pf, acc[dt]);
+      for (int dt = 0; dt < DT; ++dt) {
+        if constexpr (RW == 32) acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, li, lg), pf, acc[dt]);
+        else acc[dt] = ra_mm16<NT>(ra_read_trans16<NT, DP>(img_v, dt * 16, li, lg), pf, acc[dt]);
+      }
     }
   }
-  l += __shfl_xor(l, 32);
+#pragma unroll
+  for (int mm = RW; mm < 64; mm <<= 1) l += __shfl_xor(l, mm);
   if (!live) {                                           // rows behind the last query went along with their tile
     l = 0.f;
     m = -INFINITY;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < RW * RW / 64; ++r) acc[dt][r] = 0.f;
   }
 
-  // ---- join the four waves: maxima and sums first, then the rescaled accumulators in wave order
-  if (lk == 0) {
-    stat[wave * 32 + li] = m;
-    stat[(RA_WAVES + wave) * 32 + li] = l;
+  // ---- join the waves: maxima and sums first, then the rescaled accumulators in wave order
+  if (lg == 0) {
+    stat[wave * RW + li] = m;
+    stat[(NW + wave) * RW + li] = l;
   }
   __syncthreads();
   float mj = -INFINITY, lj = 0.f;
 #pragma unroll
-  for (int w = 0; w < RA_WAVES; ++w) mj = fmaxf(mj, stat[w * 32 + li]);
+  for (int w = 0; w < NW; ++w) mj = fmaxf(mj, stat[w * RW + li]);
   const float mz = mj == -INFINITY ? 0.f : mj;
 #pragma unroll
-  for (int w = 0; w < RA_WAVES; ++w) lj += stat[(RA_WAVES + w) * 32 + li] * ra_exp2(stat[w * 32 + li] - mz);
+  for (int w = 0; w < NW; ++w) lj += stat[(NW + w) * RW + li] * ra_exp2(stat[w * RW + li] - mz);
   const float a = ra_exp2(m - mz);
   float* jo = (float*)img_v;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      ra_store4(jo + li * (DP + 4) + dt * 32 + 8 * g + 4 * lk, acc[dt][4 * g] * a, acc[dt][4 * g + 1] * a,
+    for (int g = 0; g < RW * RW / 256; ++g)
+      ra_store4(jo + li * (DP + 4) + dt * RW + 8 * g + 4 * lg, acc[dt][4 * g] * a, acc[dt][4 * g + 1] * a,
                 acc[dt][4 * g + 2] * a, acc[dt][4 * g + 3] * a);
-  float* joined = stat + 2 * RA_WAVES * 32;
-  if (wave == 0 && lk == 0) {
+  float* joined = stat + 2 * NW * RW;
+  if (wave == 0 && lg == 0) {
     joined[li] = mj;
-    joined[32 + li] = lj;
+    joined[RW + li] = lj;
   }
   __syncthreads();
-  for (int u = tid; u < 32 * (DP / 4); u += 256) {
+  for (int u = tid; u < RW * (DP / 4); u += TH) {
     const int r = u / (DP / 4), d = (u % (DP / 4)) * 4;
-    const int rw = rt * 32 + r;
+    const int rw = rt * RW + r;
     if (rw >= rows || d >= p.D) continue;
     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < RA_WAVES; ++w) {
-      const float4 y = *(const float4*)((float*)(smem + w * RaFew<T, DP>::wave) + r * (DP + 4) + d);
+    for (int w = 0; w < NW; ++w) {
+      const float4 y = *(const float4*)((float*)(smem + w * RaFew<T, DP, RW>::wave) + r * (DP + 4) + d);
       x[0] += y.x; x[1] += y.y; x[2] += y.z; x[3] += y.w;
     }
-    const float lr = joined[32 + r], mr = joined[r];
+    const float lr = joined[RW + r], mr = joined[r];
     const int ri = rw / G, rh = hk * G + rw % G;
     if (p.part) {
-      float* ph = p.part + ((long)split * (gridDim.x / p.nsplit) + group) * (32 * (p.D + 2));
+      float* ph = p.part + (((long)unit * p.Hk + hk) * nrt + rt) * (32 * (p.D + 2));
       ra_store4(ph + 64 + r * p.D + d, x[0], x[1], x[2], x[3]);
       if (d == 0) {
         ph[r] = mr;
         ph[32 + r] = lr;
       }
     } else {
-      const float inv = lr > 0.f ? 1.0f / lr : 0.f;
+      const float inv = lr != 0.f ? 1.0f / lr : 0.f;
       ra_store4((T*)p.o + (((long)b * p.Lq + ri) * p.Hq + rh) * p.D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-      if (p.lse && d == 0) p.lse[((long)b * p.Hq + rh) * p.Lq + ri] = lr > 0.f ? mr + ra_log2(lr) : -INFINITY;
+      if (p.lse && d == 0) p.lse[((long)b * p.Hq + rh) * p.Lq + ri] = lr != 0.f ? mr + ra_log2(lr) : -INFINITY;
     }
   }
 }
 
-// joins the splits of rel_attn_few_kernel in their order: one thread four columns of a row
+// joins the parts of rel_attn_few_kernel in their order: one thread four columns of a row, a wave of one sequence
 template <class T>
-__global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p, int groups) {
+__global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
   const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
-  const int dq = p.D / 4;
-  const long u = (long)blockIdx.x * 256 + threadIdx.x;
-  const int d = (int)(u % dq) * 4;
-  const long rw_all = u / dq;
-  if (rw_all >= (long)p.B * p.Hk * rows) return;
-  const int rw = (int)(rw_all % rows);
-  const long bh = rw_all / rows;
-  const int hk = (int)(bh % p.Hk), b = (int)(bh / p.Hk);
-  const int r = rw & 31;
-  const float* ph = p.part + (bh * nrt + (rw >> 5)) * (32 * (p.D + 2));
-  const long step = (long)groups * (32 * (p.D + 2));
+  const int per = rows * (p.D / 4), blocks = (per + 255) / 256;           // four columns a thread; blocks of one key head
+  const int bh = blockIdx.x / blocks, u = (blockIdx.x - bh * blocks) * 256 + threadIdx.x;
+  const int hk = bh % p.Hk, b = bh / p.Hk;
+  int first = b * p.nsplit, n = p.nsplit;
+  if (p.by_length) {
+    int at = b, split, chunk;
+    ra_unit(p, -1, b, at, split, n, chunk);
+    first = split;
+  }
+  if (u >= per) return;
+  const int d = u % (p.D / 4) * 4, rw = u / (p.D / 4), r = rw & 31;
+  const long step = (long)p.Hk * nrt * (32 * (p.D + 2));
+  const float* ph = p.part + (((long)first * p.Hk + hk) * nrt + (rw >> 5)) * (32 * (p.D + 2));
   float m = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, ph[s * step + r]);
+#pragma unroll 8
+  for (int s = 0; s < n; ++s) m = fmaxf(m, ph[s * step + r]);
   const float mz = m == -INFINITY ? 0.f : m;
   float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < p.nsplit; ++s) {
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
     const float a = ra_exp2(ph[s * step + r] - mz);
     l = fmaf(ph[s * step + 32 + r], a, l);
     const float4 y = *(const float4*)(ph + s * step + 64 + r * p.D + d);
@@ -397,23 +503,25 @@ __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p, int grou
     x[2] = fmaf(y.z, a, x[2]);
     x[3] = fmaf(y.w, a, x[3]);
   }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
   const int i = rw / G, h = hk * G + rw % G;
   ra_store4((T*)p.o + (((long)b * p.Lq + i) * p.Hq + h) * p.D + d, x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-  if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.Lq + i] = l > 0.f ? m + ra_log2(l) : -INFINITY;
+  if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.Lq + i] = l != 0.f ? m + ra_log2(l) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// How a call is run.  The few-query kernel wins while the workgroups of the other one would not fill the card.
+// How a call is run.  The few-query kernel wins while the other one's workgroups would not be two a compute unit (4 x 2500
+// fp32 queries of 4 heads, 320 of them: 67 instead of 106 us; 252 at 3 x 777 bf16: 19 instead of 24 us).
 static void ra_plan(const int64_t* g, int& few, int& nsplit, int& chunk) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
   const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32);
-  few = rows <= 32 || B * Hq * ((Lq + 127) / 128) < 128;
+  static const long tgt = getenv("XTGT") ? atol(getenv("XTGT")) : 512;
+  few = rows <= 32 || B * Hq * ((Lq + 127) / 128) < 512;
   nsplit = 1;
   long c = Lk;
   if (few) {
     // about two workgroups a compute unit, none with less than 128 keys (a 32-key tile a wave)
-    long want = (512 + groups - 1) / groups;
+    long want = (tgt + groups - 1) / groups;
     const long most = (Lk + 127) / 128;
     want = want < 1 ? 1 : (want > most ? (most < 1 ? 1 : most) : want);
     want = want > 64 ? 64 : want;
@@ -428,12 +536,15 @@ static void ra_plan(const int64_t* g, int& few, int& nsplit, int& chunk) {
 template <class T, int DP>
 static int ra_fwd(RaParams& p, int few, void* stream) {
   if (few) {
-    const int rows = p.Lq * (p.Hq / p.Hk), groups = p.B * p.Hk * ((rows + 31) / 32);
-    const size_t lds = RA_WAVES * RaFew<T, DP>::wave + 4 * ((size_t)p.nb * 32 + 2 * p.R + 1 + (2 * RA_WAVES + 2) * 32);
-    int rc = ra_launch(rel_attn_few_kernel<T, DP>, dim3((unsigned)((long)p.nsplit * groups)), 256, lds, stream, p);
+    const long rows = (long)p.Lq * (p.Hq / p.Hk), nrt = (rows + 31) / 32;
+    const dim3 grid((unsigned)(p.units * p.Hk * nrt));
+    const int rc = rows <= 16 ? ra_launch(rel_attn_few_kernel<T, DP, 16>, grid, RaFew<T, DP, 16>::NW * 64,
+                                          RaFew<T, DP, 16>::bytes(p.nb, p.R), stream, p)
+                              : ra_launch(rel_attn_few_kernel<T, DP, 32>, grid, RaFew<T, DP, 32>::NW * 64,
+                                          RaFew<T, DP, 32>::bytes(p.nb, p.R), stream, p);
     if (rc || !p.part) return rc;
-    const long n = (long)p.B * p.Hk * rows * (p.D / 4);
-    hipLaunchKernelGGL(rel_attn_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, p, groups);
+    const long blocks = (rows * (p.D / 4) + 255) / 256;
+    hipLaunchKernelGGL(rel_attn_join_kernel<T>, dim3((unsigned)(p.B * p.Hk * blocks)), dim3(256), 0, (hipStream_t)stream, p);
     OCCF_LAUNCH_CHECK();
   }
   constexpr int NT = RaType<T>::NT, KT = NT == 3 && DP > 64 ? 32 : 64;
@@ -448,7 +559,7 @@ extern "C" long occf_rel_attn_workspace(const int64_t* geom, int dtype) {
   ra_plan(geom, few, nsplit, chunk);
   if (!few || nsplit == 1) return 0;
   const long rows = geom[1] * (geom[3] / geom[4]);
-  return (long)nsplit * geom[0] * geom[4] * ((rows + 31) / 32) * 32 * (geom[5] + 2);
+  return (long)(nsplit + 1) * geom[0] * geom[4] * ((rows + 31) / 32) * 32 * (geom[5] + 2);
 }
 
 extern "C" int occf_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
@@ -467,5 +578,7 @@ extern "C" int occf_rel_attn_fwd(const void* q, const void* k, const void* v, co
   p.q = q; p.k = k; p.v = v; p.table = table; p.lut = lut;
   p.q_lens = q_lens; p.k_lens = k_lens; p.q_start = q_start;
   p.o = out; p.lse = lse; p.part = need > 0 ? workspace : nullptr;
+  p.by_length = p.part && k_lens && p.B > 1 && p.B <= 512;
+  p.units = p.B * (p.nsplit + p.by_length);
   RA_DISPATCH(dtype, p.D, ra_fwd, p, few, stream);
 }
