@@ -652,7 +652,7 @@ int occf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_weight, co
  * zeros.  q_lens / k_lens / q_start NULL: all rows, all keys, 0.  A table entry at or below -1e30 takes its bucket out.
  * geom = { B, Lq, Lk, Hq, Hk (divides Hq: query head h reads key head h / (Hq / Hk)), D (multiple of 8, <= 128),
  *          buckets (<= 128), R (<= 512), q strides of batch / row / head, k strides, v strides } (elements, 16-byte
- * multiples; pointers 16-byte aligned).  table [buckets, Hq], lut [2 R + 1], out [B, Lq, Hq, D] contiguous,
+ * multiples; rows D or more apart; pointers 16-byte aligned).  table [buckets, Hq], lut [2 R + 1], out [B, Lq, Hq, D] contiguous,
  * lse [B, Hq, Lq] (may be NULL) = base-2 logarithm of a row's sum of exponentials (-inf: no key), what the backward reads.
  * workspace: occf_rel_attn_workspace floats (0: may be NULL; negative: arguments outside the limits). */
 long occf_rel_attn_workspace(const int64_t* geom, int dtype);

@@ -164,8 +164,7 @@ typedef uint32_t ra_u2 __attribute__((ext_vector_type(2)));
 // ---- a 4 x 4 block of a tile: 4 rows x 4 columns on their way from global memory to the LDS images
 template <class T> struct RaBlk;
 
-// bounded loads (one select on a 32-bit offset instead of a branch a load: under branches every load is waited for where the
-// paths meet).  The resource starts at the tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows
+// bounded loads (no branch a load: under branches every load is waited for where the paths meet).  The resource starts at the tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows
 // span less than 2 GiB (ra_check)
 #ifdef OCCF_EMU
 static inline RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
@@ -187,22 +186,28 @@ __device__ __forceinline__ ra_raw2 ra_buf8(occf_bbuf b, uint32_t off) {
   return __builtin_bit_cast(ra_raw2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
 }
 #endif
-__device__ __forceinline__ occf_bbuf ra_buf(const void* p) { return occf_make_bbuf(p, 0x7FFFFFFFu); }
 template <> struct RaBlk<float> { RaU4 r[4]; };
 template <> struct RaBlk<ra_bf16> { ra_raw2 r[4]; };
 
-// block u of a tile (u = row group * (DP / 4) + column group): `tile` points at row 0, rows at or behind `rows` and columns at
-// or behind D are zero; stride in elements
+// the next `rows` rows from `tile`: the resource ends with the last of them (rows lie D or more apart, ra_check), so that the
+// rows behind read as zeros without a test
+template <class T>
+__device__ __forceinline__ occf_bbuf ra_tile(const T* tile, long stride, int rows, int D) {
+  const int n = rows < 64 ? rows : 64;
+  return occf_make_bbuf(tile, n > 0 ? ((uint32_t)(n - 1) * (uint32_t)stride + (uint32_t)D) * (uint32_t)sizeof(T) : 0u);
+}
+
+// byte offset of block u of a tile (u = row group * (DP / 4) + column group); columns at or behind D lie outside any tile
 template <class T, int DP>
-__device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, const T* tile, long stride, int rows, int D, int u) {
+__device__ __forceinline__ uint32_t ra_blk_at(long stride, int D, int u) {
   const int c = (u % (DP / 4)) * 4, r0 = (u / (DP / 4)) * 4;
-  const occf_bbuf buf = ra_buf(tile);
-  const uint32_t step = (uint32_t)stride * (uint32_t)sizeof(T);
-  const uint32_t at = (uint32_t)r0 * step + (uint32_t)(c * sizeof(T));
-  const int n = c < D ? rows - r0 : 0;
+  return c < D ? ((uint32_t)r0 * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T) : OCCF_BUF_OOB;
+}
+template <class T>
+__device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, occf_bbuf buf, uint32_t at, long stride) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t off = i < n ? at + i * step : OCCF_BUF_OOB;
+    const uint32_t off = at + i * ((uint32_t)stride * (uint32_t)sizeof(T));
     if constexpr (sizeof(T) == 4) b.r[i] = ra_buf16(buf, off);
     else b.r[i] = ra_buf8(buf, off);
   }
@@ -211,12 +216,13 @@ __device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, const T* tile, long str
 // 8 columns from `c` of row `row` of such a tile, as loaded and as a fragment
 template <class T> struct RaRaw { RaU4 x[sizeof(T) / 2]; };
 template <class T>
-__device__ __forceinline__ void ra_load_raw(RaRaw<T>& f, const T* tile, long stride, int row, int rows, int c, int D) {
-  const occf_bbuf buf = ra_buf(tile);
-  const uint32_t at = (uint32_t)row * ((uint32_t)stride * (uint32_t)sizeof(T)) + (uint32_t)(c * sizeof(T));
-  const uint32_t off = row < rows && c < D ? at : OCCF_BUF_OOB;
+__device__ __forceinline__ uint32_t ra_raw_at(long stride, int D, int row, int c) {
+  return c < D ? ((uint32_t)row * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T) : OCCF_BUF_OOB;
+}
+template <class T>
+__device__ __forceinline__ void ra_load_raw(RaRaw<T>& f, occf_bbuf buf, uint32_t at) {
 #pragma unroll
-  for (int e = 0; e < (int)sizeof(T) / 2; ++e) f.x[e] = ra_buf16(buf, off + 16u * e);
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) f.x[e] = ra_buf16(buf, at + 16u * e);
 }
 __device__ __forceinline__ RaFrag<1> ra_raw_frag(const RaRaw<ra_bf16>& w) {
   RaFrag<1> f;
@@ -264,6 +270,15 @@ __device__ __forceinline__ void ra_store_row(char* img, const uint32_t (&w)[NT][
     }
 }
 
+// the low (or high) halves of two words side by side
+__device__ __forceinline__ uint32_t ra_halves(uint32_t a, uint32_t b, int high) {
+#ifdef OCCF_EMU
+  return high ? (a >> 16) | (b & 0xFFFF0000u) : (a & 0xFFFFu) | (b << 16);
+#else
+  return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
+#endif
+}
+
 template <int NT, int DP, int ROWS, int COLS = 32>
 __device__ __forceinline__ void ra_store_trans(char* img, const uint32_t (&w)[NT][4][2], int u) {
   const int c = (u % (DP / 4)) * 4, rg = u / (DP / 4);
@@ -275,14 +290,7 @@ __device__ __forceinline__ void ra_store_trans(char* img, const uint32_t (&w)[NT
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int h = j >> 1;
-      uint32_t lo, hi;
-      if (j & 1) {
-        lo = (w[t][0][h] >> 16) | (w[t][1][h] & 0xFFFF0000u);
-        hi = (w[t][2][h] >> 16) | (w[t][3][h] & 0xFFFF0000u);
-      } else {
-        lo = (w[t][0][h] & 0xFFFFu) | (w[t][1][h] << 16);
-        hi = (w[t][2][h] & 0xFFFFu) | (w[t][3][h] << 16);
-      }
+      const uint32_t lo = ra_halves(w[t][0][h], w[t][1][h], j & 1), hi = ra_halves(w[t][2][h], w[t][3][h], j & 1);
       const ra_u2 x = {lo, hi};
       *(ra_u2*)(img + t * RaTrans<ROWS>::bytes(DP) + (c + j) * RaTrans<ROWS>::LD + off) = x;
     }
@@ -417,7 +425,7 @@ static int ra_check(const int64_t* g, int dtype) {
   for (int s = 8; s < 17; ++s)
     if (g[s] < 0 || g[s] % per16) return OCCF_ESHAPE;
   for (int s = 9; s < 17; s += 3)
-    if (g[s] >= (1L << 22)) return OCCF_ESHAPE;          // 64 rows within 2 GiB
+    if (g[s] < D || g[s] >= (1L << 22)) return OCCF_ESHAPE;      // rows apart, 64 of them within 2 GiB
   return 0;
 }
 

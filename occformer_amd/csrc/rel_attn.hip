@@ -65,14 +65,22 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 
   RaBlk<T> rk[NU], rv[NU];
   const int ntile = (kend + KT - 1) / KT;
-  if (ntile > 0) {
+  uint32_t at_k[NU], at_v[NU];
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    at_k[n] = ra_blk_at<T, DP>(p.ksl, p.D, tid + n * 256);
+    at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, tid + n * 256);
+  }
+  auto load = [&](int k0) {
+    const occf_bbuf tk = ra_tile(kb + k0 * p.ksl, p.ksl, kend - k0, p.D), tv = ra_tile(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % 256 && tid + n * 256 >= NB) break;
-      ra_load_blk<T, DP>(rk[n], kb, p.ksl, kend, p.D, tid + n * 256);
-      ra_load_blk<T, DP>(rv[n], vb, p.vsl, kend, p.D, tid + n * 256);
+      ra_load_blk<T>(rk[n], tk, at_k[n], p.ksl);
+      ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
     }
-  }
+  };
+  if (ntile > 0) load(0);
   for (int kt = 0; kt < ntile; ++kt) {
     const int k0 = kt * KT;
     __syncthreads();
@@ -86,14 +94,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
       ra_store_trans<NT, DP, KT>(img_v, w, tid + n * 256);
     }
     __syncthreads();
-    if (kt + 1 < ntile) {
-#pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        if (NB % 256 && tid + n * 256 >= NB) break;
-        ra_load_blk<T, DP>(rk[n], kb + (k0 + KT) * p.ksl, p.ksl, kend - k0 - KT, p.D, tid + n * 256);
-        ra_load_blk<T, DP>(rv[n], vb + (k0 + KT) * p.vsl, p.vsl, kend - k0 - KT, p.D, tid + n * 256);
-      }
-    }
+    if (kt + 1 < ntile) load(k0 + KT);
     if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
     f32x16 s[KT / 32];
 #pragma unroll
@@ -294,15 +295,21 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
   RaRaw<T> rk[KR];
   RaBlk<T> rv[NV];
   int j0 = first + wave * 32;
-  auto load = [&](int at) {
+  uint32_t at_k[KR], at_v[NV];
 #pragma unroll
-    for (int n = 0; n < KR; ++n) {
-      const int key = RW == 32 ? li : (n / QS) * 16 + li, c = RW == 32 ? n * 16 + lg * 8 : (n % QS) * 32 + lg * 8;
-      ra_load_raw<T>(rk[n], kb + at * p.ksl, p.ksl, key, lim - at, c, p.D);
-    }
+  for (int n = 0; n < KR; ++n)
+    at_k[n] = RW == 32 ? ra_raw_at<T>(p.ksl, p.D, li, n * 16 + lg * 8)
+                       : ra_raw_at<T>(p.ksl, p.D, (n / QS) * 16 + li, (n % QS) * 32 + lg * 8);
+#pragma unroll
+  for (int n = 0; n < NV; ++n) at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, lane + n * 64);
+  auto load = [&](int j) {
+    const int left = lim - j < 32 ? lim - j : 32;
+    const occf_bbuf tk = ra_tile(kb + j * p.ksl, p.ksl, left, p.D), tv = ra_tile(vb + j * p.vsl, p.vsl, left, p.D);
+#pragma unroll
+    for (int n = 0; n < KR; ++n) ra_load_raw<T>(rk[n], tk, at_k[n]);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
-      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T, DP>(rv[n], vb + at * p.vsl, p.vsl, lim - at, p.D, lane + n * 64);
+      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
   };
   if (j0 < lim) load(j0);
 

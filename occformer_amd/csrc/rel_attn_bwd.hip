@@ -27,6 +27,8 @@
 #define RA_DFRONT 32
 #define RA_DTILE (RA_DFRONT + 16 * RA_DLD)
 
+#define RA_QSPLIT 8             // most parts of the keys that a query's walk is cut into
+
 struct RaBwd {
   RaParams a;
   void* dtable;
@@ -89,7 +91,6 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   const long stat = ((long)b * p.Hq + h) * p.Lq + ic;
   float lse = live ? p.lse[stat] : INFINITY;
   if (lse == -INFINITY) lse = INFINITY;                  // no key: P = 0
-  if (i < p.Lq && lk == 0 && split == 0) p.delta[stat] = delta;
   const f32x16 s_first = ra_splat16(-lse / p.c), dp_first = ra_splat16(-delta);
 
   int kend = nk;
@@ -111,12 +112,19 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   RaBlk<T> rk[NU], rv[NU];
   const int ntile = (kend + KT - 1) / KT;
   const int t0 = (int)((long)ntile * split / g.qsplit), t1 = (int)((long)ntile * (split + 1) / g.qsplit);
+  uint32_t at_k[NU], at_v[NU];
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    at_k[n] = ra_blk_at<T, DP>(p.ksl, p.D, tid + n * TH);
+    at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, tid + n * TH);
+  }
   auto load = [&](int k0) {
+    const occf_bbuf tk = ra_tile(kb + k0 * p.ksl, p.ksl, kend - k0, p.D), tv = ra_tile(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T, DP>(rk[n], kb + k0 * p.ksl, p.ksl, kend - k0, p.D, tid + n * TH);
-      ra_load_blk<T, DP>(rv[n], vb + k0 * p.vsl, p.vsl, kend - k0, p.D, tid + n * TH);
+      ra_load_blk<T>(rk[n], tk, at_k[n], p.ksl);
+      ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
     }
   };
   if (t0 < t1) load(t0 * KT);
@@ -173,7 +181,9 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   }
   eps += __shfl_xor(eps, 32);
   if (i >= p.Lq) return;
-  if (lk == 0) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;
+  // one part: the corrected delta; several: the parts' sums, delta among the first one's
+  if (lk == 0) p.delta[(long)split * p.B * p.Hq * p.Lq + stat] = split == 0 ? delta + eps : eps;
+  if (lk == 0 && g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;
   const long part = (long)split * p.B * p.Lq * p.Hq * p.D + orow;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -275,35 +285,44 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   }
   float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
   RaBlk<T> rq[NU], ro[NU];
-  float nlse = 0.f, ndelta = 0.f;
-  auto load = [&](int step) {
-    const int h = hk * G + step / ntile, r0 = first + (step % ntile) * QT;
-    const T* qb = (const T*)p.q + (long)b * p.qsb + (long)h * p.qsh;
-    const T* ob = (const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D;
+  // the next tile's rows, and on QT lanes their statistics, all looked at only when the tile is stored: a value that is used
+  // where it is loaded would make the workgroup wait for it in every step
+  float nlse = 0.f, ndelta[RA_QSPLIT];
+  uint32_t at_q[NU], at_o[NU];
+  const long osl = (long)p.Hq * p.D;
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    at_q[n] = ra_blk_at<T, DP>(p.qsl, p.D, tid + n * TH);
+    at_o[n] = ra_blk_at<T, DP>(osl, p.D, tid + n * TH);
+  }
+  auto load = [&](int hg, int r0) {
+    const int h = hk * G + hg;
+    const occf_bbuf tq = ra_tile((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nq - r0, p.D);
+    const occf_bbuf to = ra_tile((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nq - r0, p.D);
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T, DP>(rq[n], qb + r0 * p.qsl, p.qsl, nq - r0, p.D, tid + n * TH);
-      ra_load_blk<T, DP>(ro[n], ob + (long)r0 * p.Hq * p.D, (long)p.Hq * p.D, nq - r0, p.D, tid + n * TH);
+      ra_load_blk<T>(rq[n], tq, at_q[n], p.qsl);
+      ra_load_blk<T>(ro[n], to, at_o[n], osl);
     }
     if (tid < QT) {
-      const int i = r0 + tid;
-      const long stat = ((long)b * p.Hq + h) * p.Lq + i;
-      nlse = INFINITY;
-      ndelta = 0.f;
-      if (i < nq) {
-        const float x = p.lse[stat];
-        nlse = x == -INFINITY ? INFINITY : x;
-        ndelta = p.delta[stat];
-        for (int s = 0; s < g.qsplit; ++s) ndelta += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
-      }
+      const long stat = ((long)b * p.Hq + h) * p.Lq + occf_clampi(r0 + tid, p.Lq - 1);
+      nlse = p.lse[stat];
+#pragma unroll
+      for (int s = 0; s < RA_QSPLIT; ++s)
+        if (s < g.qsplit) ndelta[s] = p.delta[(long)s * p.B * p.Hq * p.Lq + stat];
     }
   };
-  if (t0 < t1) load(t0);
-  for (int step = t0; step < t1; ++step) {
-    const int hg = step / ntile, r0 = first + (step - hg * ntile) * QT;
+  int hg = t0 < t1 ? t0 / ntile : 0, at = t0 - hg * ntile;                // head of the group and query tile of a step
+  if (t0 < t1) load(hg, first + at * QT);
+  for (int step = t0; step < t1; ++step, ++at) {
+    if (at == ntile) {
+      at = 0;
+      ++hg;
+    }
+    const int r0 = first + at * QT;
     __syncthreads();
-    if (step == t0 || step == hg * ntile) ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
+    if (step == t0 || at == 0) ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       if (NB % TH && tid + n * TH >= NB) break;
@@ -316,11 +335,17 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       ra_store_trans<NT, DP, QT>(img_ot, w, tid + n * TH);
     }
     if (tid < QT) {
-      s_lse[tid] = -nlse / p.c;
-      s_delta[tid] = -ndelta;
+      // rows that do not count or see no key: P = 0
+      const bool row = r0 + tid < nq;
+      s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : -nlse / p.c;
+      float x = ndelta[0];
+#pragma unroll
+      for (int s = 1; s < RA_QSPLIT; ++s)
+        if (s < g.qsplit) x += ndelta[s];
+      s_delta[tid] = row ? -x : 0.f;
     }
     __syncthreads();
-    if (step + 1 < t1) load(step + 1);
+    if (step + 1 < t1) load(at + 1 < ntile ? hg : hg + 1, at + 1 < ntile ? r0 + QT : first);
 #pragma unroll
     for (int sub = 0; sub < QT / 32; ++sub) {
       const int i0 = r0 + sub * 32, rel0 = j0 - (start + i0);
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
         }
       }
     }
-    if (step + 1 == t1 || step + 1 == (hg + 1) * ntile) {
+    if (step + 1 == t1 || at + 1 == ntile) {
       // a head is done: its distances' sums, waves in order, then the buckets', distances in order
 #pragma unroll
       for (int mm = 32; mm > 0; mm >>= 1) {
@@ -512,14 +537,15 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// How often the walks are cut: until about four workgroups a compute unit are there, in steps of two or more tiles.
+// How often the walks are cut: until about two workgroups a compute unit are there (what its registers hold), 128 rows or more
+// a part.
 static void ra_bwd_plan(const int64_t* g, int& qsplit, int& ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
   const long wq = B * Hq * ((Lq + 127) / 128), wk = B * Hk * ((Lk + 127) / 128);
   const long mq = (Lk + 127) / 128, mk = (Hq / Hk) * ((Lq + 127) / 128);
   const auto cut = [](long want, long most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
-  qsplit = wq >= 512 ? 1 : cut(cut(1024 / wq, mq), 16);
-  ksplit = wk >= 512 ? 1 : cut(cut(1024 / wk, mk), 16);
+  qsplit = cut(cut(512 / wq, mq), RA_QSPLIT);
+  ksplit = cut(cut((512 + wk / 2) / wk, mk), 16);
 }
 
 struct RaBwdSizes { long delta, eps, dq, dk, tab; };
@@ -527,8 +553,8 @@ static RaBwdSizes ra_bwd_sizes(const int64_t* g, int dtype, int qsplit, int kspl
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6];
   RaBwdSizes s;
   const auto up = [](long n) { return (n + 63) / 64 * 64; };             // parts start on 256 bytes
-  s.delta = up(B * Hq * Lq);
-  s.eps = up(B * Hq * Lq * qsplit);
+  s.delta = up(B * Hq * Lq * qsplit);
+  s.eps = qsplit > 1 ? s.delta : 0;
   s.dq = qsplit > 1 ? up(B * Lq * Hq * D * qsplit) : 0;
   s.dk = ksplit > 1 ? up(B * Lk * Hk * D * ksplit) : 0;
   s.tab = up(B * Hq * ksplit * ((Lk + 127) / 128) * nb);

@@ -1319,7 +1319,8 @@ class HipOps:
     def _aligned(t):
         """``t`` itself where its rows can be read 16 bytes at a time, else a copy"""
         per16 = 16 // t.element_size()
-        if t.data_ptr() % 16 or any(s % per16 for s in t.stride()[:-1]) or t.stride(1) >= 1 << 22:
+        if t.data_ptr() % 16 or any(s % per16 for s in t.stride()[:-1]) or \
+                not t.shape[3] <= t.stride(1) < 1 << 22:
             return t.clone(memory_format=torch.contiguous_format)
         return t
 
