@@ -3,8 +3,9 @@
 // Both directions are written on 32 x 32 score tiles of v_mfma_f32_32x32x16_bf16 in the orientation that keeps the
 // scores in registers: the accumulator of one product is the B operand of the next.  A lane holds ONE column of the tile
 // (lane & 31) and 16 of its 32 rows, row(r) = (r & 3) + 8 (r >> 2) + 4 (lane >> 5); registers 0..7 are then a B operand of
-// 16 k-values {4 lk + 0..3, 8 + 4 lk + 0..3}, registers 8..15 the next 16.  The A operand of that second product is read
-// from a TRANSPOSED image of the tile whose 4-row groups are stored in the same order (ra_store_trans).
+// 16 k-values {4 lk + 0..3, 8 + 4 lk + 0..3}, registers 8..15 the next 16.  The A operand of that second product is the tile
+// transposed: ds_read_b64_tr_b16 hands the lanes of a 16-lane group one column each of a 4 x 16 block of the row image, in just
+// this order, so that a tile lies in LDS once, as rows.
 //
 // Products: bf16 inputs are one product.  fp32 inputs are split into three bf16 pieces (x = h + m + l, 24 bits) and a
 // product is the six terms above 2^-24; the two-piece, three-term form the other attention kernels use leaves 3e-6 ... 5e-6
@@ -146,49 +147,28 @@ __device__ __forceinline__ void ra_store4(ra_bf16* p, float a, float b, float c,
   *(U2*)__builtin_assume_aligned(p, 8) = U2{occf_bf16_pack2(a, b), occf_bf16_pack2(c, d)};
 }
 
-// LDS images of a tile of ROWS x DP, one per piece.
-//   row image:   [ROWS][DP], 16 bytes of padding a row: the 16-lane groups of a b128 read hit 16 different bank quads
-//   trans image: [DP][ROWS], 4-row groups in operand order, 16 bytes of padding, the 16-byte slots of a row exchanged by
-//                (column >> 4) & 3 so that the 16 column groups of a store do not meet on one bank quad
+// LDS image of a tile's rows, one per piece.  The stride is an odd number of 16-byte units, so that the 16 rows of a b128 read lie
+// on different bank quads; 304 for 128 columns (not 272), so that the 8 rows x 64 bytes of a transposing read spread over all 64
+// banks too.
 template <int DP> struct RaRow {
-  static constexpr int LD = DP * 2 + 16;
+  static constexpr int LD = DP == 128 ? 304 : DP * 2 + 16;
   static constexpr int bytes(int rows) { return rows * LD; }
-};
-template <int ROWS> struct RaTrans {
-  static constexpr int LD = ROWS * 2 + 16;
-  static constexpr int bytes(int dp) { return dp * LD; }
 };
 
 typedef uint32_t ra_u2 __attribute__((ext_vector_type(2)));
 
-// ---- a 4 x 4 block of a tile: 4 rows x 4 columns on their way from global memory to the LDS images
-template <class T> struct RaBlk;
-
-// bounded loads (no branch a load: under branches every load is waited for where the paths meet).  The resource starts at the tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows
-// span less than 2 GiB (ra_check)
+// bounded loads (no branch a load: under branches every load is waited for where the paths meet).  The resource starts at the
+// tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows span less than 2 GiB (ra_check)
 #ifdef OCCF_EMU
 static inline RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
   const occf_u32x4 v = occf_bbuf_load_b128(b, off);
   return RaU4{{v.x, v.y, v.z, v.w}};
 }
-struct ra_raw2 { uint32_t x, y; };
-static inline ra_raw2 ra_buf8(occf_bbuf b, uint32_t off) {
-  ra_raw2 v = {0u, 0u};
-  if ((uint64_t)off + 8u <= (uint64_t)b.nbytes) memcpy(&v, b.base + off, 8);
-  return v;
-}
 #else
 __device__ __forceinline__ RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
   return __builtin_bit_cast(RaU4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
 }
-struct ra_raw2 { uint32_t x, y; };
-__device__ __forceinline__ ra_raw2 ra_buf8(occf_bbuf b, uint32_t off) {
-  return __builtin_bit_cast(ra_raw2, __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, 0));
-}
 #endif
-template <> struct RaBlk<float> { RaU4 r[4]; };
-template <> struct RaBlk<ra_bf16> { ra_raw2 r[4]; };
-
 // the next `rows` rows from `tile`: the resource ends with the last of them (rows lie D or more apart, ra_check), so that the
 // rows behind read as zeros without a test
 template <class T>
@@ -197,21 +177,46 @@ __device__ __forceinline__ occf_bbuf ra_tile(const T* tile, long stride, int row
   return occf_make_bbuf(tile, n > 0 ? ((uint32_t)(n - 1) * (uint32_t)stride + (uint32_t)D) * (uint32_t)sizeof(T) : 0u);
 }
 
-// byte offset of block u of a tile (u = row group * (DP / 4) + column group); columns at or behind D lie outside any tile
-template <class T, int DP>
-__device__ __forceinline__ uint32_t ra_blk_at(long stride, int D, int u) {
-  const int c = (u % (DP / 4)) * 4, r0 = (u / (DP / 4)) * 4;
-  return c < D ? ((uint32_t)r0 * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T) : OCCF_BUF_OOB;
-}
-template <class T>
-__device__ __forceinline__ void ra_load_blk(RaBlk<T>& b, occf_bbuf buf, uint32_t at, long stride) {
+// A tile of ROWS x DP in 16-byte pieces of rows, NU of them a thread of TH: byte offsets (columns at or behind D lie outside any
+// tile), loads, and the way into the row image
+template <class T, int DP, int ROWS, int TH>
+struct RaTileRegs {
+  static constexpr int C = 16 / sizeof(T), PER = DP / C, NB = ROWS * PER, NU = (NB + TH - 1) / TH, NT = RaType<T>::NT;
+  RaU4 x[NU];
+  uint32_t at[NU];
+  __device__ __forceinline__ void place(long stride, int D, int tid) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t off = at + i * ((uint32_t)stride * (uint32_t)sizeof(T));
-    if constexpr (sizeof(T) == 4) b.r[i] = ra_buf16(buf, off);
-    else b.r[i] = ra_buf8(buf, off);
+    for (int n = 0; n < NU; ++n) {
+      const int u = tid + n * TH, row = u / PER, c = (u % PER) * C;
+      at[n] = c < D && u < NB ? ((uint32_t)row * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T) : OCCF_BUF_OOB;
+    }
   }
-}
+  __device__ __forceinline__ void load(const T* tile, long stride, int rows, int D) {
+    const occf_bbuf buf = ra_tile(tile, stride, rows < ROWS ? rows : ROWS, D);
+#pragma unroll
+    for (int n = 0; n < NU; ++n) x[n] = ra_buf16(buf, at[n]);
+  }
+  __device__ __forceinline__ void store(char* img, int tid) const {
+#pragma unroll
+    for (int n = 0; n < NU; ++n) {
+      const int u = tid + n * TH, row = u / PER, c = (u % PER) * C;
+      if (NB % TH && u >= NB) break;
+      char* to = img + row * RaRow<DP>::LD + c * 2;
+      if constexpr (NT == 1) {
+        *(bf16x8*)to = ra_as_frag(x[n].x[0], x[n].x[1], x[n].x[2], x[n].x[3]);
+      } else {
+        uint32_t a[3], b[3];
+        ra_split2<3>(occf_u2f(x[n].x[0]), occf_u2f(x[n].x[1]), a);
+        ra_split2<3>(occf_u2f(x[n].x[2]), occf_u2f(x[n].x[3]), b);
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+          const ra_u2 w = {a[t], b[t]};
+          *(ra_u2*)(to + t * RaRow<DP>::bytes(ROWS)) = w;
+        }
+      }
+    }
+  }
+};
 
 // 8 columns from `c` of row `row` of such a tile, as loaded and as a fragment
 template <class T> struct RaRaw { RaU4 x[sizeof(T) / 2]; };
@@ -236,65 +241,23 @@ __device__ __forceinline__ RaFrag<3> ra_raw_frag(const RaRaw<float>& w) {
   return ra_pack8<3>(f);
 }
 
-// block -> packed pieces, w[piece][row][pair of columns]
-__device__ __forceinline__ void ra_blk_pieces(const RaBlk<ra_bf16>& b, uint32_t (&w)[1][4][2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[0][i][0] = b.r[i].x;
-    w[0][i][1] = b.r[i].y;
-  }
-}
-__device__ __forceinline__ void ra_blk_pieces(const RaBlk<float>& b, uint32_t (&w)[3][4][2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t s[3];
-    ra_split2<3>(occf_u2f(b.r[i].x[0]), occf_u2f(b.r[i].x[1]), s);
-#pragma unroll
-    for (int t = 0; t < 3; ++t) w[t][i][0] = s[t];
-    ra_split2<3>(occf_u2f(b.r[i].x[2]), occf_u2f(b.r[i].x[3]), s);
-#pragma unroll
-    for (int t = 0; t < 3; ++t) w[t][i][1] = s[t];
-  }
-}
-
-
-template <int NT, int DP, int ROWS>
-__device__ __forceinline__ void ra_store_row(char* img, const uint32_t (&w)[NT][4][2], int u) {
-  const int c = (u % (DP / 4)) * 4, rg = u / (DP / 4);
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const ra_u2 x = {w[t][i][0], w[t][i][1]};
-      *(ra_u2*)(img + t * RaRow<DP>::bytes(ROWS) + (rg * 4 + i) * RaRow<DP>::LD + c * 2) = x;
-    }
-}
-
-// the low (or high) halves of two words side by side
-__device__ __forceinline__ uint32_t ra_halves(uint32_t a, uint32_t b, int high) {
+// ds_read_b64_tr_b16: lane 4 r + q of a 16-lane group gives the address of row r, columns 4 q .. 4 q + 3 of a 4 x 16 block;
+// lane t gets column t, rows 0..3
 #ifdef OCCF_EMU
-  return high ? (a >> 16) | (b & 0xFFFF0000u) : (a & 0xFFFFu) | (b << 16);
+static inline ra_u2 ra_read_tr(const char* at) {
+  struct V { uint16_t e[4]; } v;
+  memcpy(&v, at, 8);
+  const int lane = threadIdx.x & 63, t = lane & 15;
+  uint32_t r[4];
+  for (int e = 0; e < 4; ++e) r[e] = hipemu::lane_exchange(v, (lane & 48) + 4 * e + (t >> 2)).e[t & 3];
+  return ra_u2{r[0] | (r[1] << 16), r[2] | (r[3] << 16)};
+}
 #else
-  return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
+typedef short ra_s4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ ra_u2 ra_read_tr(const char* at) {
+  return __builtin_bit_cast(ra_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) ra_s4*)at));
+}
 #endif
-}
-
-template <int NT, int DP, int ROWS, int COLS = 32>
-__device__ __forceinline__ void ra_store_trans(char* img, const uint32_t (&w)[NT][4][2], int u) {
-  const int c = (u % (DP / 4)) * 4, rg = u / (DP / 4);
-  // row group g of a 16-row step holds k values lk = g & 1, e = 4 (g >> 1) ..: 8-byte slot 2 lk + (g >> 1)
-  const int g = rg & 3, slot = COLS == 16 ? g : (rg >> 2) * 2 + (g & 1), half = COLS == 16 ? rg >> 2 : g >> 1;
-  const int off = ((slot ^ ((c >> 4) & 3)) * 16) + half * 8;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int h = j >> 1;
-      const uint32_t lo = ra_halves(w[t][0][h], w[t][1][h], j & 1), hi = ra_halves(w[t][2][h], w[t][3][h], j & 1);
-      const ra_u2 x = {lo, hi};
-      *(ra_u2*)(img + t * RaTrans<ROWS>::bytes(DP) + (c + j) * RaTrans<ROWS>::LD + off) = x;
-    }
-}
 
 // A operand: 32 rows from row0, k step ks of 16 columns
 template <int NT, int DP, int ROWS>
@@ -305,31 +268,34 @@ __device__ __forceinline__ RaFrag<NT> ra_read_row(const char* img, int row0, int
     f.p[t] = *(const bf16x8*)(img + t * RaRow<DP>::bytes(ROWS) + (row0 + li) * RaRow<DP>::LD + ks * 32 + lk * 16);
   return f;
 }
-// A operand of the 16-column form: 16 columns of the tile from c0, its 32 rows; g = lane >> 4
-template <int NT, int DP>
-__device__ __forceinline__ RaFrag<NT> ra_read_trans16(const char* img, int c0, int li, int g) {
+// A operand, transposed: 32 columns of the tile from c0, k step ks of 16 tile rows
+template <int NT, int DP, int ROWS>
+__device__ __forceinline__ RaFrag<NT> ra_read_trans(const char* img, int c0, int ks, int lane) {
   RaFrag<NT> f;
-  const int d = c0 + li;
+  const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  const char* at = img + row * RaRow<DP>::LD + col * 2 + ks * 16 * RaRow<DP>::LD + c0 * 2;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    f.p[t] = *(const bf16x8*)(img + t * RaTrans<32>::bytes(DP) + d * RaTrans<32>::LD + ((g ^ ((d >> 4) & 3)) * 16));
+  for (int t = 0; t < NT; ++t) {
+    const ra_u2 a = ra_read_tr(at + t * RaRow<DP>::bytes(ROWS)), b = ra_read_tr(at + t * RaRow<DP>::bytes(ROWS) + 8 * RaRow<DP>::LD);
+    f.p[t] = ra_as_frag(a.x, a.y, b.x, b.y);
+  }
   return f;
 }
-// A operand: 32 columns of the tile from c0, k step ks of 16 tile rows
-template <int NT, int DP, int ROWS>
-__device__ __forceinline__ RaFrag<NT> ra_read_trans(const char* img, int c0, int ks, int li, int lk) {
+// the same for the 16-column form: 16 columns of the tile from c0, its 32 rows
+template <int NT, int DP>
+__device__ __forceinline__ RaFrag<NT> ra_read_trans16(const char* img, int c0, int lane) {
   RaFrag<NT> f;
-  const int d = c0 + li;
+  const char* at = img + (4 * (lane >> 4) + ((lane & 15) >> 2)) * RaRow<DP>::LD + (c0 + 4 * (lane & 3)) * 2;
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    f.p[t] = *(const bf16x8*)(img + t * RaTrans<ROWS>::bytes(DP) + d * RaTrans<ROWS>::LD +
-                              (((ks * 2 + lk) ^ ((d >> 4) & 3)) * 16));
+  for (int t = 0; t < NT; ++t) {
+    const ra_u2 a = ra_read_tr(at + t * RaRow<DP>::bytes(32)), b = ra_read_tr(at + t * RaRow<DP>::bytes(32) + 16 * RaRow<DP>::LD);
+    f.p[t] = ra_as_frag(a.x, a.y, b.x, b.y);
+  }
   return f;
 }
 
 // ---- the same chain on 16 columns (v_mfma_f32_16x16x32_bf16): a lane holds column lane & 15 and, of 32 tile rows in two
-// accumulators, rows 16 (e >> 2) + 4 (lane >> 4) + (e & 3), e = 0..7, which are one B operand of 32 k-values; the transposed
-// image keeps row group g = row >> 2 at 16-byte slot g & 3, half g >> 2.
+// accumulators, rows 16 (e >> 2) + 4 (lane >> 4) + (e & 3), e = 0..7, which are one B operand of 32 k-values.
 template <int NT>
 __device__ __forceinline__ f32x4 ra_mm16(const RaFrag<NT>& a, const RaFrag<NT>& b, f32x4 c) {
   if constexpr (NT == 3) {

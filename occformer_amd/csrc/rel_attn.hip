@@ -16,15 +16,20 @@
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Many queries: a workgroup owns 128 queries of one head, a wave 32 of them (a lane one query: its running maximum and sum
-// are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.
+// are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.  With two
+// images (NBUF) a tile costs one barrier: the next one is stored while the others still read this one.
+template <class T, int DP, int KT>
+struct RaFwd {
+  static constexpr int tile = 2 * RaType<T>::NT * RaRow<DP>::bytes(KT);                  // K and V
+  static constexpr int NBUF = tile <= 32 * 1024 ? 2 : 1;
+  static size_t bytes(int R) { return NBUF * tile + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
+};
+
 template <class T, int DP, int KT>
 __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) rel_attn_fwd_kernel(RaParams p) {
-  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
-  constexpr int NB = KT * DP / 16, NU = (NB + 255) / 256;               // 4 x 4 blocks of a tile, and a thread's share
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, NBUF = RaFwd<T, DP, KT>::NBUF;
   OCCF_DYN_SMEM(smem);
-  char* img_k = smem;
-  char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
-  float* lut = (float*)(img_v + NT * RaTrans<KT>::bytes(DP));
+  float* lut = (float*)(smem + NBUF * RaFwd<T, DP, KT>::tile);
 
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
   const int nqt = (p.Lq + 127) / 128;
@@ -63,38 +68,38 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
   for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
   float m = -INFINITY, mref = 0.f, l = 0.f;
 
-  RaBlk<T> rk[NU], rv[NU];
-  const int ntile = (kend + KT - 1) / KT;
-  uint32_t at_k[NU], at_v[NU];
-#pragma unroll
-  for (int n = 0; n < NU; ++n) {
-    at_k[n] = ra_blk_at<T, DP>(p.ksl, p.D, tid + n * 256);
-    at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, tid + n * 256);
-  }
-  auto load = [&](int k0) {
-    const occf_bbuf tk = ra_tile(kb + k0 * p.ksl, p.ksl, kend - k0, p.D), tv = ra_tile(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % 256 && tid + n * 256 >= NB) break;
-      ra_load_blk<T>(rk[n], tk, at_k[n], p.ksl);
-      ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
-    }
+  RaTileRegs<T, DP, KT, 256> rk, rv;
+  rk.place(p.ksl, p.D, tid);
+  rv.place(p.vsl, p.D, tid);
+  const auto load = [&](int k0) {
+    rk.load(kb + k0 * p.ksl, p.ksl, kend - k0, p.D);
+    rv.load(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
   };
-  if (ntile > 0) load(0);
+  const auto store = [&](int buf) {
+    rk.store(smem + buf * RaFwd<T, DP, KT>::tile, tid);
+    rv.store(smem + buf * RaFwd<T, DP, KT>::tile + NT * RaRow<DP>::bytes(KT), tid);
+  };
+  const int ntile = (kend + KT - 1) / KT;
+  if (ntile > 0) {
+    load(0);
+    if (NBUF == 2) {
+      store(0);
+      if (ntile > 1) load(KT);
+    }
+  }
   for (int kt = 0; kt < ntile; ++kt) {
     const int k0 = kt * KT;
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % 256 && tid + n * 256 >= NB) break;
-      uint32_t w[NT][4][2];
-      ra_blk_pieces(rk[n], w);
-      ra_store_row<NT, DP, KT>(img_k, w, tid + n * 256);
-      ra_blk_pieces(rv[n], w);
-      ra_store_trans<NT, DP, KT>(img_v, w, tid + n * 256);
+    __syncthreads();                                     // this tile is stored, and no wave reads the one before it any more
+    if (NBUF == 1) {
+      store(0);
+      __syncthreads();
+      if (kt + 1 < ntile) load(k0 + KT);
+    } else if (kt + 1 < ntile) {
+      store((kt + 1) & 1);
+      if (kt + 2 < ntile) load(k0 + 2 * KT);
     }
-    __syncthreads();
-    if (kt + 1 < ntile) load(k0 + KT);
+    const char* img_k = smem + (NBUF == 2 ? kt & 1 : 0) * RaFwd<T, DP, KT>::tile;
+    const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
     if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
     f32x16 s[KT / 32];
 #pragma unroll
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
         const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-          acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, KT>(img_v, dt * 32, sub * 2 + s2, li, lk), pf, acc[dt]);
+          acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, KT>(img_v, dt * 32, sub * 2 + s2, lane), pf, acc[dt]);
       }
     }
   }
@@ -218,14 +223,14 @@ __device__ __forceinline__ bool ra_unit(const RaParams& p, int unit, int seq, in
 
 // Few queries: the rows of one key head (query i of its G query heads, row = i G + g) in groups of RW = 32, or 16 where there are
 // no more, share every key that is read.  The keys are split over workgroups and, tile by tile, over a workgroup's four waves;
-// a wave reads its key rows straight into operand registers and turns its value rows round in LDS of its own, so that no wave
+// a wave reads its key rows straight into operand registers and takes its value rows through LDS of its own, so that no wave
 // waits for another before the join at the end.  (Keys through LDS, in whole rows of the cache line, took 99 instead of 67 us for
 // 4 x 2500 fp32 queries and as long for single ones.)  Bound by the stream of keys and values: 16 rows take half the
 // accumulators, products and exponentials of 32, which leaves room for a second tile in flight.
 // part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
 template <class T, int DP, int RW>
 struct RaFew {
-  static constexpr int NT = RaType<T>::NT, NW = 4, VT = NT * RaTrans<32>::bytes(DP);
+  static constexpr int NT = RaType<T>::NT, NW = 4, VT = NT * RaRow<DP>::bytes(32);
   static constexpr int join = RW * (DP + 4) * 4;         // [RW rows][DP + 4] floats of one wave
   static constexpr int wave = VT > join ? VT : join;
   static size_t bytes(int nb, int R) { return NW * wave + 4 * ((size_t)nb * RW + 2 * R + 1 + (2 * NW + 2) * RW); }
@@ -239,7 +244,6 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
   constexpr int QS = DP / (RW == 32 ? 16 : 32);          // k steps of Q K^T
   constexpr int KR = DP / 16;                            // key fragments: [k step] or [16-key half][k step]
   constexpr int DT = DP / RW;                            // column tiles of the output
-  constexpr int NB = 2 * DP, NV = (NB + 63) / 64;        // 4 x 4 blocks of 32 value rows, and a lane's share
   typedef typename std::conditional<RW == 32, f32x16, f32x4>::type Acc;
   OCCF_DYN_SMEM(smem);
   const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & (RW - 1), lg = lane / RW;
@@ -293,23 +297,19 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
 
   // the first tile is on its way before the tables are made
   RaRaw<T> rk[KR];
-  RaBlk<T> rv[NV];
+  RaTileRegs<T, DP, 32, 64> rv;
+  rv.place(p.vsl, p.D, lane);
   int j0 = first + wave * 32;
-  uint32_t at_k[KR], at_v[NV];
+  uint32_t at_k[KR];
 #pragma unroll
   for (int n = 0; n < KR; ++n)
     at_k[n] = RW == 32 ? ra_raw_at<T>(p.ksl, p.D, li, n * 16 + lg * 8)
                        : ra_raw_at<T>(p.ksl, p.D, (n / QS) * 16 + li, (n % QS) * 32 + lg * 8);
-#pragma unroll
-  for (int n = 0; n < NV; ++n) at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, lane + n * 64);
   auto load = [&](int j) {
-    const int left = lim - j < 32 ? lim - j : 32;
-    const occf_bbuf tk = ra_tile(kb + j * p.ksl, p.ksl, left, p.D), tv = ra_tile(vb + j * p.vsl, p.vsl, left, p.D);
+    const occf_bbuf tk = ra_tile(kb + j * p.ksl, p.ksl, lim - j < 32 ? lim - j : 32, p.D);
 #pragma unroll
     for (int n = 0; n < KR; ++n) ra_load_raw<T>(rk[n], tk, at_k[n]);
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (NB % 64 == 0 || lane + n * 64 < NB) ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
+    rv.load(vb + j * p.vsl, p.vsl, lim - j, p.D);
   };
   if (j0 < lim) load(j0);
 
@@ -338,13 +338,7 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
 
   for (; j0 < lim; j0 += NW * 32) {
     RA_WAVE_SYNC();
-#pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (NB % 64 == 0 || lane + n * 64 < NB) {
-        uint32_t w[NT][4][2];
-        ra_blk_pieces(rv[n], w);
-        ra_store_trans<NT, DP, 32, RW>(img_v, w, lane + n * 64);
-      }
+    rv.store(img_v, lane);
     RA_WAVE_SYNC();
     float s[NE];
     if constexpr (RW == 32) {
@@ -409,8 +403,8 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
       const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (RW == 32) acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, li, lg), pf, acc[dt]);
-        else acc[dt] = ra_mm16<NT>(ra_read_trans16<NT, DP>(img_v, dt * 16, li, lg), pf, acc[dt]);
+        if constexpr (RW == 32) acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, lane), pf, acc[dt]);
+        else acc[dt] = ra_mm16<NT>(ra_read_trans16<NT, DP>(img_v, dt * 16, lane), pf, acc[dt]);
       }
     }
   }
@@ -555,7 +549,7 @@ static int ra_fwd(RaParams& p, int few, void* stream) {
     OCCF_LAUNCH_CHECK();
   }
   constexpr int NT = RaType<T>::NT, KT = NT == 3 && DP > 64 ? 32 : 64;
-  const size_t lds = NT * (RaRow<DP>::bytes(KT) + RaTrans<KT>::bytes(DP)) + 4 * (2 * (size_t)p.R + 1 + 2 * RA_PAD);
+  const size_t lds = RaFwd<T, DP, KT>::bytes(p.R);
   return ra_launch(rel_attn_fwd_kernel<T, DP, KT>, dim3((unsigned)((long)p.B * p.Hq * ((p.Lq + 127) / 128))), 256, lds,
                    stream, p);
 }

@@ -38,22 +38,18 @@ struct RaBwd {
 
 template <class T, int DP, int KT>
 struct RaDq {
-  static constexpr int NT = RaType<T>::NT;
-  static constexpr int images = NT * (2 * RaRow<DP>::bytes(KT) + RaTrans<KT>::bytes(DP));
-  static size_t bytes(int R) { return images + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
+  static constexpr int tile = 2 * RaType<T>::NT * RaRow<DP>::bytes(KT);                  // K and V
+  static constexpr int NBUF = tile <= 32 * 1024 ? 2 : 1;                                 // (see rel_attn_fwd_kernel)
+  static size_t bytes(int R) { return NBUF * tile + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
 };
 
 template <class T, int DP, int KT, int NW>
 __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq_kernel(RaBwd g) {
   const RaParams& p = g.a;
-  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, QW = NW * 32;
-  constexpr int NB = KT * DP / 16, NU = (NB + TH - 1) / TH;
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, QW = NW * 32, NBUF = RaDq<T, DP, KT>::NBUF;
   constexpr bool PK = NT == 1;
   OCCF_DYN_SMEM(smem);
-  char* img_k = smem;
-  char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
-  char* img_kt = img_v + NT * RaRow<DP>::bytes(KT);
-  float* lut = (float*)(img_kt + NT * RaTrans<KT>::bytes(DP));
+  float* lut = (float*)(smem + NBUF * RaDq<T, DP, KT>::tile);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
 
   const int nqt = (p.Lq + QW - 1) / QW;
@@ -109,40 +105,39 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   for (int dt = 0; dt < (PK ? DT : 1); ++dt) pk[dt] = ra_zero16();
   float eps = 0.f;
 
-  RaBlk<T> rk[NU], rv[NU];
+  RaTileRegs<T, DP, KT, TH> rk, rv;
+  rk.place(p.ksl, p.D, tid);
+  rv.place(p.vsl, p.D, tid);
   const int ntile = (kend + KT - 1) / KT;
   const int t0 = (int)((long)ntile * split / g.qsplit), t1 = (int)((long)ntile * (split + 1) / g.qsplit);
-  uint32_t at_k[NU], at_v[NU];
-#pragma unroll
-  for (int n = 0; n < NU; ++n) {
-    at_k[n] = ra_blk_at<T, DP>(p.ksl, p.D, tid + n * TH);
-    at_v[n] = ra_blk_at<T, DP>(p.vsl, p.D, tid + n * TH);
-  }
-  auto load = [&](int k0) {
-    const occf_bbuf tk = ra_tile(kb + k0 * p.ksl, p.ksl, kend - k0, p.D), tv = ra_tile(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T>(rk[n], tk, at_k[n], p.ksl);
-      ra_load_blk<T>(rv[n], tv, at_v[n], p.vsl);
-    }
+  const auto load = [&](int k0) {
+    rk.load(kb + k0 * p.ksl, p.ksl, kend - k0, p.D);
+    rv.load(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
   };
-  if (t0 < t1) load(t0 * KT);
+  const auto store = [&](int buf) {
+    rk.store(smem + buf * RaDq<T, DP, KT>::tile, tid);
+    rv.store(smem + buf * RaDq<T, DP, KT>::tile + NT * RaRow<DP>::bytes(KT), tid);
+  };
+  if (t0 < t1) {
+    load(t0 * KT);
+    if (NBUF == 2) {
+      store(0);
+      if (t0 + 1 < t1) load((t0 + 1) * KT);
+    }
+  }
   for (int kt = t0; kt < t1; ++kt) {
     const int k0 = kt * KT;
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % TH && tid + n * TH >= NB) break;
-      uint32_t w[NT][4][2];
-      ra_blk_pieces(rk[n], w);
-      ra_store_row<NT, DP, KT>(img_k, w, tid + n * TH);
-      ra_store_trans<NT, DP, KT>(img_kt, w, tid + n * TH);
-      ra_blk_pieces(rv[n], w);
-      ra_store_row<NT, DP, KT>(img_v, w, tid + n * TH);
+    if (NBUF == 1) {
+      store(0);
+      __syncthreads();
+      if (kt + 1 < t1) load(k0 + KT);
+    } else if (kt + 1 < t1) {
+      store((kt + 1 - t0) & 1);
+      if (kt + 2 < t1) load(k0 + 2 * KT);
     }
-    __syncthreads();
-    if (kt + 1 < t1) load(k0 + KT);
+    const char* img_k = smem + (NBUF == 2 ? (kt - t0) & 1 : 0) * RaDq<T, DP, KT>::tile;
+    const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
     if (i0 >= nq) continue;                              // wave-uniform
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
@@ -172,7 +167,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
         const RaFrag<NT> df = ra_pack8<NT>(ds + s2 * 8), pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const RaFrag<NT> kt_f = ra_read_trans<NT, DP, KT>(img_kt, dt * 32, sub * 2 + s2, li, lk);
+          const RaFrag<NT> kt_f = ra_read_trans<NT, DP, KT>(img_k, dt * 32, sub * 2 + s2, lane);
           acc[dt] = ra_mm<NT>(kt_f, df, acc[dt]);
           if (PK) pk[dt] = ra_mm<NT>(kt_f, pf, pk[dt]);
         }
@@ -209,26 +204,19 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
 
 template <class T, int DP, int QT, int NW>
 struct RaDkv {
-  static constexpr int NT = RaType<T>::NT;
-  static constexpr int images = 2 * NT * (RaRow<DP>::bytes(QT) + RaTrans<QT>::bytes(DP));
-  static size_t bytes(int R) {
-    return images + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + 2 * QT + NW * RA_DTILE);
-  }
+  static constexpr int images = 2 * RaType<T>::NT * RaRow<DP>::bytes(QT);                // Q and dO
+  static constexpr int tile = images + 2 * QT * 4;                                       // and the rows' statistics
+  static constexpr int NBUF = tile <= 20 * 1024 ? 2 : 1;                                 // (see rel_attn_fwd_kernel)
+  static size_t bytes(int R) { return NBUF * tile + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + NW * RA_DTILE); }
 };
 
 template <class T, int DP, int QT, int NW>
 __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dkv_kernel(RaBwd g) {
   const RaParams& p = g.a;
-  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, KW = NW * 32;
-  constexpr int NB = QT * DP / 16, NU = (NB + TH - 1) / TH;
+  typedef RaDkv<T, DP, QT, NW> L;
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, KW = NW * 32, NBUF = L::NBUF;
   OCCF_DYN_SMEM(smem);
-  char* img_q = smem;
-  char* img_o = img_q + NT * RaRow<DP>::bytes(QT);
-  char* img_qt = img_o + NT * RaRow<DP>::bytes(QT);
-  char* img_ot = img_qt + NT * RaTrans<QT>::bytes(DP);
-  float* s_lse = (float*)(img_ot + NT * RaTrans<QT>::bytes(DP));       // first values of the accumulators' rows
-  float* s_delta = s_lse + QT;
-  float* tiles = s_delta + QT;
+  float* tiles = (float*)(smem + NBUF * L::tile);
   float* lut = tiles + NW * RA_DTILE;
   const int nl = 2 * p.R + 1 + 2 * RA_PAD;
   float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
@@ -284,27 +272,20 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     dv[dt] = ra_zero16();
   }
   float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
-  RaBlk<T> rq[NU], ro[NU];
+  RaTileRegs<T, DP, QT, TH> rq, ro;
+  const long osl = (long)p.Hq * p.D;
+  rq.place(p.qsl, p.D, tid);
+  ro.place(osl, p.D, tid);
   // the next tile's rows, and on QT lanes their statistics, all looked at only when the tile is stored: a value that is used
   // where it is loaded would make the workgroup wait for it in every step
   float nlse = 0.f, ndelta[RA_QSPLIT];
-  uint32_t at_q[NU], at_o[NU];
-  const long osl = (long)p.Hq * p.D;
-#pragma unroll
-  for (int n = 0; n < NU; ++n) {
-    at_q[n] = ra_blk_at<T, DP>(p.qsl, p.D, tid + n * TH);
-    at_o[n] = ra_blk_at<T, DP>(osl, p.D, tid + n * TH);
-  }
-  auto load = [&](int hg, int r0) {
-    const int h = hk * G + hg;
-    const occf_bbuf tq = ra_tile((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nq - r0, p.D);
-    const occf_bbuf to = ra_tile((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nq - r0, p.D);
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % TH && tid + n * TH >= NB) break;
-      ra_load_blk<T>(rq[n], tq, at_q[n], p.qsl);
-      ra_load_blk<T>(ro[n], to, at_o[n], osl);
-    }
+  int hg = t0 < t1 ? t0 / ntile : 0, at = t0 - hg * ntile;               // head of the group and query tile of a step
+  int lhg = hg, lat = at;                                                // ... of the next load
+  int nrow = 0;                                                          // the loaded tile's first query
+  const auto load = [&]() {
+    const int h = hk * G + lhg, r0 = first + lat * QT;
+    rq.load((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nq - r0, p.D);
+    ro.load((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nq - r0, p.D);
     if (tid < QT) {
       const long stat = ((long)b * p.Hq + h) * p.Lq + occf_clampi(r0 + tid, p.Lq - 1);
       nlse = p.lse[stat];
@@ -312,31 +293,21 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       for (int s = 0; s < RA_QSPLIT; ++s)
         if (s < g.qsplit) ndelta[s] = p.delta[(long)s * p.B * p.Hq * p.Lq + stat];
     }
+    nrow = r0;
+    if (++lat == ntile) {
+      lat = 0;
+      ++lhg;
+    }
   };
-  int hg = t0 < t1 ? t0 / ntile : 0, at = t0 - hg * ntile;                // head of the group and query tile of a step
-  if (t0 < t1) load(hg, first + at * QT);
-  for (int step = t0; step < t1; ++step, ++at) {
-    if (at == ntile) {
-      at = 0;
-      ++hg;
-    }
-    const int r0 = first + at * QT;
-    __syncthreads();
-    if (step == t0 || at == 0) ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
-#pragma unroll
-    for (int n = 0; n < NU; ++n) {
-      if (NB % TH && tid + n * TH >= NB) break;
-      uint32_t w[NT][4][2];
-      ra_blk_pieces(rq[n], w);
-      ra_store_row<NT, DP, QT>(img_q, w, tid + n * TH);
-      ra_store_trans<NT, DP, QT>(img_qt, w, tid + n * TH);
-      ra_blk_pieces(ro[n], w);
-      ra_store_row<NT, DP, QT>(img_o, w, tid + n * TH);
-      ra_store_trans<NT, DP, QT>(img_ot, w, tid + n * TH);
-    }
+  // s_lse, s_delta: first values of the accumulators' rows
+  const auto store = [&](int buf) {
+    char* to = smem + buf * L::tile;
+    rq.store(to, tid);
+    ro.store(to + NT * RaRow<DP>::bytes(QT), tid);
+    float *s_lse = (float*)(to + L::images), *s_delta = s_lse + QT;
     if (tid < QT) {
       // rows that do not count or see no key: P = 0
-      const bool row = r0 + tid < nq;
+      const bool row = nrow + tid < nq;
       s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : -nlse / p.c;
       float x = ndelta[0];
 #pragma unroll
@@ -344,8 +315,36 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
         if (s < g.qsplit) x += ndelta[s];
       s_delta[tid] = row ? -x : 0.f;
     }
+  };
+  if (t0 < t1) {
+    load();
+    if (NBUF == 2) {
+      store(0);
+      if (t0 + 1 < t1) load();
+    }
+  }
+  for (int step = t0; step < t1; ++step, ++at) {
+    if (at == ntile) {
+      at = 0;
+      ++hg;
+    }
+    const int r0 = first + at * QT;
     __syncthreads();
-    if (step + 1 < t1) load(at + 1 < ntile ? hg : hg + 1, at + 1 < ntile ? r0 + QT : first);
+    if (step == t0 || at == 0) {
+      ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
+      if (NBUF == 2) __syncthreads();
+    }
+    if (NBUF == 1) {
+      store(0);
+      __syncthreads();
+      if (step + 1 < t1) load();
+    } else if (step + 1 < t1) {
+      store((step + 1 - t0) & 1);
+      if (step + 2 < t1) load();
+    }
+    const char* img_q = smem + (NBUF == 2 ? (step - t0) & 1 : 0) * L::tile;
+    const char* img_o = img_q + NT * RaRow<DP>::bytes(QT);
+    const float *s_lse = (const float*)(img_q + L::images), *s_delta = s_lse + QT;
 #pragma unroll
     for (int sub = 0; sub < QT / 32; ++sub) {
       const int i0 = r0 + sub * 32, rel0 = j0 - (start + i0);
@@ -402,8 +401,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
         const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8), df = ra_pack8<NT>(ds + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_ot, dt * 32, sub * 2 + s2, li, lk), pf, dv[dt]);
-          dk[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_qt, dt * 32, sub * 2 + s2, li, lk), df, dk[dt]);
+          dv[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_o, dt * 32, sub * 2 + s2, lane), pf, dv[dt]);
+          dk[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_q, dt * 32, sub * 2 + s2, lane), df, dk[dt]);
         }
       }
     }
@@ -538,18 +537,18 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // How often the walks are cut: until about two workgroups a compute unit are there (what its registers hold), 128 rows or more
-// a part.
-static void ra_bwd_plan(const int64_t* g, int& qsplit, int& ksplit) {
+// a part; twice as many of a causal walk's unequal key tiles (275 instead of 374 us at 2 x 4096, 4 key heads of 64).
+static void ra_bwd_plan(const int64_t* g, int causal, int& qsplit, int& ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
   const long wq = B * Hq * ((Lq + 127) / 128), wk = B * Hk * ((Lk + 127) / 128);
   const long mq = (Lk + 127) / 128, mk = (Hq / Hk) * ((Lq + 127) / 128);
   const auto cut = [](long want, long most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
   qsplit = cut(cut(512 / wq, mq), RA_QSPLIT);
-  ksplit = cut(cut((512 + wk / 2) / wk, mk), 16);
+  ksplit = cut(cut(((causal ? 1024 : 512) + wk / 2) / wk, mk), 16);
 }
 
 struct RaBwdSizes { long delta, eps, dq, dk, tab; };
-static RaBwdSizes ra_bwd_sizes(const int64_t* g, int dtype, int qsplit, int ksplit) {
+static RaBwdSizes ra_bwd_sizes(const int64_t* g, int qsplit, int ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6];
   RaBwdSizes s;
   const auto up = [](long n) { return (n + 63) / 64 * 64; };             // parts start on 256 bytes
@@ -558,7 +557,6 @@ static RaBwdSizes ra_bwd_sizes(const int64_t* g, int dtype, int qsplit, int kspl
   s.dq = qsplit > 1 ? up(B * Lq * Hq * D * qsplit) : 0;
   s.dk = ksplit > 1 ? up(B * Lk * Hk * D * ksplit) : 0;
   s.tab = up(B * Hq * ksplit * ((Lk + 127) / 128) * nb);
-  (void)dtype;
   return s;
 }
 
@@ -581,11 +579,11 @@ static int ra_bwd(const RaBwd& g, void* stream) {
   OCCF_LAUNCH_CHECK();
 }
 
-extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int dtype) {
+extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype) {
   if (ra_check(geom, dtype)) return -1;
   int qs, ks;
-  ra_bwd_plan(geom, qs, ks);
-  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, qs, ks);
+  ra_bwd_plan(geom, causal, qs, ks);
+  const RaBwdSizes s = ra_bwd_sizes(geom, qs, ks);
   return s.delta + s.eps + s.dq * (dtype == 1 ? 2 : 1) + s.dk * 2 + s.tab;
 }
 
@@ -601,7 +599,7 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)dout | (uintptr_t)workspace | (uintptr_t)dq | (uintptr_t)dk |
         (uintptr_t)dv) & 15) != 0)
     return OCCF_EINVAL;
-  if (workspace_floats < occf_rel_attn_bwd_workspace(geom, dtype)) return OCCF_EINVAL;
+  if (workspace_floats < occf_rel_attn_bwd_workspace(geom, causal, dtype)) return OCCF_EINVAL;
   RaBwd g = {};
   g.a = ra_params(geom, scale, causal);
   RaParams& p = g.a;
@@ -610,8 +608,8 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
   p.out = out; p.dout = dout; p.lse = (float*)lse;
   p.dq = dq; p.dk = dk; p.dv = dv;
   g.dtable = dtable;
-  ra_bwd_plan(geom, g.qsplit, g.ksplit);
-  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, g.qsplit, g.ksplit);
+  ra_bwd_plan(geom, causal, g.qsplit, g.ksplit);
+  const RaBwdSizes s = ra_bwd_sizes(geom, g.qsplit, g.ksplit);
   p.delta = workspace;
   g.eps = p.delta + s.delta;
   g.dq_part = g.eps + s.eps;

@@ -1391,7 +1391,7 @@ class HipOps:
         dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
         dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
         dtable = torch.empty_like(table)
-        need = self.lib.occf_rel_attn_bwd_workspace(geom, dt)
+        need = self.lib.occf_rel_attn_bwd_workspace(geom, int(bool(causal)), dt)
         if need < 0:
             raise OccfError(f"{what}: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
         ws = torch.empty((need,), dtype=self.f32, device=q.device)

@@ -479,7 +479,7 @@ def test_rel_attention_c_entry_refuses(be):
         g = list(good)
         g[at] = value
         assert lib.occf_rel_attn_workspace((ctypes.c_int64 * 17)(*g), 1) == -1
-        assert lib.occf_rel_attn_bwd_workspace((ctypes.c_int64 * 17)(*g), 1) == -1
+        assert lib.occf_rel_attn_bwd_workspace((ctypes.c_int64 * 17)(*g), 0, 1) == -1
     g = (ctypes.c_int64 * 17)(*good)
     assert lib.occf_rel_attn_workspace(g, 2) == -1 and lib.occf_rel_attn_workspace(g, 0) >= 0
     assert lib.occf_rel_attn_fwd(n, n, n, n, n, n, n, n, n, n, n, 0, g, 1.0, 0, 0, n) < 0
