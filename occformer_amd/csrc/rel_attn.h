@@ -19,6 +19,7 @@
 #ifdef OCCF_EMU
 #define ra_mfma16(a, b, c) emu_mfma_f32_16x16x32_bf16(a, b, c)
 #define RA_WAVE_SYNC() hipemu::wave_sync()
+#define RA_WAIT_LOADS() do { } while (0)
 static inline float ra_exp2(float x) { return exp2f(x); }
 static inline float ra_log2(float x) { return log2f(x); }
 #else
@@ -32,6 +33,10 @@ typedef __bf16 ra_bf16x8 __attribute__((ext_vector_type(8)));
     __builtin_amdgcn_wave_barrier();                      \
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront"); \
   } while (0)
+// every load so far has arrived.  Operands that a loop keeps are loaded, then waited for, in front of it: left to the first use
+// inside, the wait is repeated in every round and takes the next tile's loads with it.  No branch stands between such loads and
+// the loop (tiles behind the last are loaded as no rows), or the wait is found missing on a path that is never taken
+#define RA_WAIT_LOADS() __builtin_amdgcn_s_waitcnt(0x0F70)             // vmcnt(0)
 __device__ __forceinline__ float ra_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ra_log2(float x) { return __builtin_amdgcn_logf(x); }
 #endif
@@ -164,9 +169,17 @@ static inline RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
   const occf_u32x4 v = occf_bbuf_load_b128(b, off);
   return RaU4{{v.x, v.y, v.z, v.w}};
 }
+static inline float ra_buf4(occf_bbuf b, uint32_t off) {
+  float v = 0.f;
+  if ((uint64_t)off + 4u <= (uint64_t)b.nbytes) memcpy(&v, b.base + off, 4);
+  return v;
+}
 #else
 __device__ __forceinline__ RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
   return __builtin_bit_cast(RaU4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+__device__ __forceinline__ float ra_buf4(occf_bbuf b, uint32_t off) {
+  return occf_u2f(__builtin_amdgcn_raw_buffer_load_b32(b, off, 0, 0));
 }
 #endif
 // the next `rows` rows from `tile`: the resource ends with the last of them (rows lie D or more apart, ra_check), so that the
@@ -182,11 +195,13 @@ __device__ __forceinline__ occf_bbuf ra_tile(const T* tile, long stride, int row
 template <class T, int DP, int ROWS, int TH>
 struct RaTileRegs {
   static constexpr int C = 16 / sizeof(T), PER = DP / C, NB = ROWS * PER, NU = (NB + TH - 1) / TH, NT = RaType<T>::NT;
+  // whole rows a step of the workgroup: the pieces of a thread lie a constant apart
+  static constexpr bool EVEN = TH % PER == 0;
   RaU4 x[NU];
-  uint32_t at[NU];
+  uint32_t at[EVEN ? 1 : NU];
   __device__ __forceinline__ void place(long stride, int D, int tid) {
 #pragma unroll
-    for (int n = 0; n < NU; ++n) {
+    for (int n = 0; n < (EVEN ? 1 : NU); ++n) {
       const int u = tid + n * TH, row = u / PER, c = (u % PER) * C;
       at[n] = c < D && u < NB ? ((uint32_t)row * (uint32_t)stride + (uint32_t)c) * (uint32_t)sizeof(T) : OCCF_BUF_OOB;
     }
@@ -194,7 +209,8 @@ struct RaTileRegs {
   __device__ __forceinline__ void load(const T* tile, long stride, int rows, int D) {
     const occf_bbuf buf = ra_tile(tile, stride, rows < ROWS ? rows : ROWS, D);
 #pragma unroll
-    for (int n = 0; n < NU; ++n) x[n] = ra_buf16(buf, at[n]);
+    for (int n = 0; n < NU; ++n)
+      x[n] = ra_buf16(buf, EVEN ? at[0] + n * (TH / PER) * ((uint32_t)stride * (uint32_t)sizeof(T)) : at[EVEN ? 0 : n]);
   }
   __device__ __forceinline__ void store(char* img, int tid) const {
 #pragma unroll
@@ -374,6 +390,9 @@ __device__ __forceinline__ void ra_lengths(const RaParams& p, int b, int& nq, in
   nk = p.k_lens ? occf_clampi(p.k_lens[b], p.Lk) : p.Lk;
   start = p.q_start ? p.q_start[b] : 0;
   start = start < -(1 << 29) ? -(1 << 29) : (start > (1 << 29) ? (1 << 29) : start);      // distances fit 32 bits
+  nq = occf_wave_uniform(nq);                            // scalar loop bounds and branches
+  nk = occf_wave_uniform(nk);
+  start = occf_wave_uniform(start);
 }
 
 // ---- host side
@@ -386,7 +405,7 @@ static int ra_check(const int64_t* g, int dtype) {
   if (Lk > (1L << 29) || Lq > (1L << 29) || B * Hq * ((Lq + 31) / 32) * 16 >= 2147483647L ||
       B * Hk * ((Lk + 127) / 128) * 16 >= 2147483647L)
     return OCCF_ESHAPE;
-  if (Lq * (Hq / Hk) >= (1L << 30) || B * Hk * ((Lq * (Hq / Hk) + 31) / 32) * 64 >= 2147483647L) return OCCF_ESHAPE;
+  if (Hq * Lq >= (1L << 29) || Lq * (Hq / Hk) >= (1L << 30) || B * Hk * ((Lq * (Hq / Hk) + 31) / 32) * 64 >= 2147483647L) return OCCF_ESHAPE;
   const long per16 = dtype == 0 ? 4 : 8;
   for (int s = 8; s < 17; ++s)
     if (g[s] < 0 || g[s] % per16) return OCCF_ESHAPE;

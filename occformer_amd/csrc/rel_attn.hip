@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
   OCCF_DYN_SMEM(smem);
   float* lut = (float*)(smem + NBUF * RaFwd<T, DP, KT>::tile);
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & 31, lk = lane >> 5;
   const int nqt = (p.Lq + 127) / 128;
   int qt, bh;
   ra_order(p, blockIdx.x, nqt, p.B * p.Hq, qt, bh);
@@ -80,12 +80,11 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
     rv.store(smem + buf * RaFwd<T, DP, KT>::tile + NT * RaRow<DP>::bytes(KT), tid);
   };
   const int ntile = (kend + KT - 1) / KT;
-  if (ntile > 0) {
-    load(0);
-    if (NBUF == 2) {
-      store(0);
-      if (ntile > 1) load(KT);
-    }
+  load(0);
+  RA_WAIT_LOADS();
+  if (NBUF == 2) {
+    store(0);
+    load(KT);
   }
   for (int kt = 0; kt < ntile; ++kt) {
     const int k0 = kt * KT;
@@ -93,10 +92,10 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
     if (NBUF == 1) {
       store(0);
       __syncthreads();
-      if (kt + 1 < ntile) load(k0 + KT);
-    } else if (kt + 1 < ntile) {
+      load(k0 + KT);
+    } else {
       store((kt + 1) & 1);
-      if (kt + 2 < ntile) load(k0 + 2 * KT);
+      load(k0 + 2 * KT);
     }
     const char* img_k = smem + (NBUF == 2 ? kt & 1 : 0) * RaFwd<T, DP, KT>::tile;
     const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
@@ -311,7 +310,7 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
     for (int n = 0; n < KR; ++n) ra_load_raw<T>(rk[n], tk, at_k[n]);
     rv.load(vb + j * p.vsl, p.vsl, lim - j, p.D);
   };
-  if (j0 < lim) load(j0);
+  load(j0);
 
   const T* qrow = (const T*)p.q + (long)b * p.qsb + (long)(live ? i : 0) * p.qsl + (long)(live ? h : 0) * p.qsh;
   RaFrag<NT> qf[QS];
@@ -320,6 +319,7 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
     const int d = (ks * (64 / RW) + lg) * 8;
     qf[ks] = ra_row_frag<T>(qrow + (d < p.D ? d : 0), live && d < p.D);
   }
+  RA_WAIT_LOADS();
   if (first < lim) {
     for (int t = tid; t < p.nb * RW; t += TH) {
       const int r = rt * RW + t % RW;
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
         for (int e = 0; e < 4; ++e) s[hf * 4 + e] = x[e];
       }
     }
-    if (j0 + NW * 32 < lim) load(j0 + NW * 32);
+    load(j0 + NW * 32);
 
     const int lo = j0 - (start + i_last), hi = j0 + 31 - (start + i_first);        // distances of the tile
     float mx = -INFINITY;

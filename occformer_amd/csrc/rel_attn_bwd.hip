@@ -9,7 +9,7 @@
 //   rel_attn_dkv_kernel  a wave owns 32 keys (lane = key) and walks the queries of every head that shares them:
 //                        S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS, and the distances' sums of dS
 // The scores are formed twice: 7 products instead of 5, where a single pass would have to add dQ up across workgroups.
-// -lse / c and -delta are the accumulators' first values, so that neither costs an instruction a score.
+// -delta (and -lse / c where it is a row's, not a lane's) is the accumulators' first value: no instruction a score.
 //
 // delta: a row of dS sums to zero, but <dO, O> of an O rounded to bf16 (whose P was rounded too) is off by a few 2^-9, and the
 // bias' gradient, sums of dS that nearly cancel, shows it (3.5e-3 of error where its own rounding is 1.7e-3).  The row sums of
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   constexpr bool PK = NT == 1;
   OCCF_DYN_SMEM(smem);
   float* lut = (float*)(smem + NBUF * RaDq<T, DP, KT>::tile);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & 31, lk = lane >> 5;
 
   const int nqt = (p.Lq + QW - 1) / QW;
   int qt, bh;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   const long stat = ((long)b * p.Hq + h) * p.Lq + ic;
   float lse = live ? p.lse[stat] : INFINITY;
   if (lse == -INFINITY) lse = INFINITY;                  // no key: P = 0
-  const f32x16 s_first = ra_splat16(-lse / p.c), dp_first = ra_splat16(-delta);
+  const f32x16 dp_first = ra_splat16(-delta);
 
   int kend = nk;
   if (p.causal) {
@@ -118,12 +118,11 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     rk.store(smem + buf * RaDq<T, DP, KT>::tile, tid);
     rv.store(smem + buf * RaDq<T, DP, KT>::tile + NT * RaRow<DP>::bytes(KT), tid);
   };
-  if (t0 < t1) {
-    load(t0 * KT);
-    if (NBUF == 2) {
-      store(0);
-      if (t0 + 1 < t1) load((t0 + 1) * KT);
-    }
+  load(t0 * KT);
+  RA_WAIT_LOADS();
+  if (NBUF == 2) {
+    store(0);
+    load((t0 + 1) * KT);
   }
   for (int kt = t0; kt < t1; ++kt) {
     const int k0 = kt * KT;
@@ -131,10 +130,10 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     if (NBUF == 1) {
       store(0);
       __syncthreads();
-      if (kt + 1 < t1) load(k0 + KT);
-    } else if (kt + 1 < t1) {
+      load(k0 + KT);
+    } else {
       store((kt + 1 - t0) & 1);
-      if (kt + 2 < t1) load(k0 + 2 * KT);
+      load(k0 + 2 * KT);
     }
     const char* img_k = smem + (NBUF == 2 ? (kt - t0) & 1 : 0) * RaDq<T, DP, KT>::tile;
     const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
@@ -143,7 +142,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= kend || (p.causal && rel0 > 31)) continue;
-      f32x16 s = s_first, dp = dp_first;
+      f32x16 s = ra_zero16(), dp = dp_first;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s);
@@ -155,6 +154,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
       ra_bias_mask<1>(s, lut + (near ? jl - pi + p.R + RA_PAD : 0), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
                       j0 + 32 > kend || (p.causal && rel0 + 31 > 0), p.c, ce, be,
                       [&](int o) { return jl + o >= kend || (p.causal && jl + o > pi); });
+      be -= lse;
       float ds[16], pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -202,6 +202,13 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     }
 }
 
+// one statistic of a row: array [parts][B][Hq][Lq], byte offset `at` within the batch entry; `ok` false: 0
+__device__ __forceinline__ float ra_load_stat(const float* x, const RaParams& p, int b, int part, uint32_t at, bool ok) {
+  const long n = (long)p.Hq * p.Lq;
+  const occf_bbuf buf = occf_make_bbuf(x + ((long)part * p.B + b) * n, (uint32_t)n * 4u);
+  return ra_buf4(buf, ok ? at : OCCF_BUF_OOB);
+}
+
 template <class T, int DP, int QT, int NW>
 struct RaDkv {
   static constexpr int images = 2 * RaType<T>::NT * RaRow<DP>::bytes(QT);                // Q and dO
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   float* lut = tiles + NW * RA_DTILE;
   const int nl = 2 * p.R + 1 + 2 * RA_PAD;
   float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 31, lk = lane >> 5;
+  const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & 31, lk = lane >> 5;
   float* dsum = sums + wave * nl;
   float* tile = tiles + wave * RA_DTILE + RA_DFRONT;
   for (int t = tid; t < NW * RA_DTILE; t += TH) tiles[t] = 0.f;
@@ -280,20 +287,21 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   // where it is loaded would make the workgroup wait for it in every step
   float nlse = 0.f, ndelta[RA_QSPLIT];
   int hg = t0 < t1 ? t0 / ntile : 0, at = t0 - hg * ntile;               // head of the group and query tile of a step
-  int lhg = hg, lat = at;                                                // ... of the next load
-  int nrow = 0;                                                          // the loaded tile's first query
+  int lstep = t0, lhg = hg, lat = at;                                    // ... of the next load
+  int nrow = 0, nend = 0;                                                // the loaded tile's first query, and behind its last
   const auto load = [&]() {
-    const int h = hk * G + lhg, r0 = first + lat * QT;
-    rq.load((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nq - r0, p.D);
-    ro.load((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nq - r0, p.D);
-    if (tid < QT) {
-      const long stat = ((long)b * p.Hq + h) * p.Lq + occf_clampi(r0 + tid, p.Lq - 1);
-      nlse = p.lse[stat];
-#pragma unroll
-      for (int s = 0; s < RA_QSPLIT; ++s)
-        if (s < g.qsplit) ndelta[s] = p.delta[(long)s * p.B * p.Hq * p.Lq + stat];
-    }
+    const bool more = lstep < t1;                                        // (else: no rows)
+    const int h = hk * G + (more ? lhg : 0), r0 = more ? first + lat * QT : 0;
     nrow = r0;
+    nend = more ? nq : 0;
+    rq.load((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nend - r0, p.D);
+    ro.load((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nend - r0, p.D);
+    const uint32_t stat = ((uint32_t)h * (uint32_t)p.Lq + (uint32_t)(r0 + tid)) * 4u;
+    nlse = ra_load_stat(p.lse, p, b, 0, stat, tid < QT && r0 + tid < nend);
+#pragma unroll
+    for (int s = 0; s < RA_QSPLIT; ++s)
+      if (s < g.qsplit) ndelta[s] = ra_load_stat(p.delta, p, b, s, stat, tid < QT && r0 + tid < nend);
+    ++lstep;
     if (++lat == ntile) {
       lat = 0;
       ++lhg;
@@ -307,7 +315,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     float *s_lse = (float*)(to + L::images), *s_delta = s_lse + QT;
     if (tid < QT) {
       // rows that do not count or see no key: P = 0
-      const bool row = nrow + tid < nq;
+      const bool row = nrow + tid < nend;
       s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : -nlse / p.c;
       float x = ndelta[0];
 #pragma unroll
@@ -316,12 +324,11 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       s_delta[tid] = row ? -x : 0.f;
     }
   };
-  if (t0 < t1) {
+  load();
+  RA_WAIT_LOADS();
+  if (NBUF == 2) {
+    store(0);
     load();
-    if (NBUF == 2) {
-      store(0);
-      if (t0 + 1 < t1) load();
-    }
   }
   for (int step = t0; step < t1; ++step, ++at) {
     if (at == ntile) {
@@ -337,10 +344,10 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     if (NBUF == 1) {
       store(0);
       __syncthreads();
-      if (step + 1 < t1) load();
-    } else if (step + 1 < t1) {
+      load();
+    } else {
       store((step + 1 - t0) & 1);
-      if (step + 2 < t1) load();
+      load();
     }
     const char* img_q = smem + (NBUF == 2 ? (step - t0) & 1 : 0) * L::tile;
     const char* img_o = img_q + NT * RaRow<DP>::bytes(QT);
