@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_dw_kernel(const float* __res
   const float* src = part + (which ? (long)nq * D : 0);
   float sum = 0.f;
   if (c < D)
+#pragma unroll 8
     for (int i = r; i < n; i += 32) sum += src[(long)i * D + c];
   acc[r][threadIdx.x & 7] = sum;
   __syncthreads();
@@ -281,7 +282,7 @@ static int qn_setup(QnParams& p, const void* q, const void* k, const void* qw, c
   p.s[1] = QnSide{k, nullptr, kw, nullptr, g[14], g[15], g[16], (int)Hk, 0};
   const long rpb = 256 / lpr;
   for (int i = 0; i < 2; ++i) {
-    const long n = (B * L * (i ? Hk : Hq) + rpb - 1) / rpb, most = bwd ? 1024 : 8192;
+    const long n = (B * L * (i ? Hk : Hq) + rpb - 1) / rpb, most = bwd ? 512 : 8192;
     p.s[i].blocks = (int)(n < most ? n : most);
   }
   return 0;
@@ -319,7 +320,7 @@ extern "C" int occf_qk_norm_rope_fwd(const void* q, const void* k, const void* q
   OCCF_LAUNCH_CHECK();
 }
 
-extern "C" long occf_qk_norm_rope_bwd_workspace(int head_dim) { return 2048L * head_dim; }
+extern "C" long occf_qk_norm_rope_bwd_workspace(int head_dim) { return 1024L * head_dim; }
 
 extern "C" int occf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
                                      const float* cos, const float* sin, const int32_t* positions, const void* dq_out,

@@ -20,6 +20,7 @@
 #define ra_mfma16(a, b, c) emu_mfma_f32_16x16x32_bf16(a, b, c)
 #define RA_WAVE_SYNC() hipemu::wave_sync()
 #define RA_WAIT_LOADS() do { } while (0)
+#define RA_PRIO(n) do { } while (0)
 static inline float ra_exp2(float x) { return exp2f(x); }
 static inline float ra_log2(float x) { return log2f(x); }
 #else
@@ -37,6 +38,8 @@ typedef __bf16 ra_bf16x8 __attribute__((ext_vector_type(8)));
 // inside, the wait is repeated in every round and takes the next tile's loads with it.  No branch stands between such loads and
 // the loop (tiles behind the last are loaded as no rows), or the wait is found missing on a path that is never taken
 #define RA_WAIT_LOADS() __builtin_amdgcn_s_waitcnt(0x0F70)             // vmcnt(0)
+// the wave that has products to issue goes first, so that the matrix pipe works while another wave of the SIMD does its scores
+#define RA_PRIO(n) __builtin_amdgcn_s_setprio(n)
 __device__ __forceinline__ float ra_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float ra_log2(float x) { return __builtin_amdgcn_logf(x); }
 #endif
@@ -337,6 +340,18 @@ __device__ __forceinline__ void ra_fill_bias(float* lut, const RaParams& p, int 
     const int b = occf_clampi(p.lut[d], p.nb - 1);
     lut[i] = ra_bias(ra_to_float(table[(long)b * p.Hq + h]));
   }
+}
+
+// biases of head h behind either end of the distances
+template <class T>
+__device__ __forceinline__ void ra_far_bias(const RaParams& p, int h, float& below, float& above) {
+  const T* table = (const T*)p.table;
+  below = ra_bias(ra_to_float(table[(long)occf_clampi(p.lut[0], p.nb - 1) * p.Hq + h]));
+  above = ra_bias(ra_to_float(table[(long)occf_clampi(p.lut[2 * p.R], p.nb - 1) * p.Hq + h]));
+#ifndef OCCF_EMU
+  below = occf_u2f(occf_wave_uniform(occf_f2u(below)));
+  above = occf_u2f(occf_wave_uniform(occf_f2u(above)));
+#endif
 }
 
 // Bias and mask of a lane's 16 raw scores s, in place.  The biased base-2 score of entry r is then fma(s[r], ce, be): a tile

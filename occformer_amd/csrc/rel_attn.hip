@@ -42,6 +42,15 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
   ra_lengths(p, b, nq, nk, start);
 
   ra_fill_bias<T>(lut, p, h, tid, 256);
+  float far_below, far_above;
+  ra_far_bias<T>(p, h, far_below, far_above);
+
+  const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
+  const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
+
+  RaTileRegs<T, DP, KT, 256> rk, rv;
+  rk.place(p.ksl, p.D, tid);
+  rv.place(p.vsl, p.D, tid);
 
   const int i0 = qt * 128 + wave * 32, i = i0 + li;
   const int pi = start + i;
@@ -60,17 +69,11 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
     kend = last < kend ? (last > 0 ? last : 0) : kend;
   }
   if (qt * 128 >= nq) kend = 0;
-  const T* kb = (const T*)p.k + (long)b * p.ksb + (long)hk * p.ksh;
-  const T* vb = (const T*)p.v + (long)b * p.vsb + (long)hk * p.vsh;
-
   f32x16 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
   float m = -INFINITY, mref = 0.f, l = 0.f;
 
-  RaTileRegs<T, DP, KT, 256> rk, rv;
-  rk.place(p.ksl, p.D, tid);
-  rv.place(p.vsl, p.D, tid);
   const auto load = [&](int k0) {
     rk.load(kb + k0 * p.ksl, p.ksl, kend - k0, p.D);
     rv.load(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
@@ -101,6 +104,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
     const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
     if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
     f32x16 s[KT / 32];
+    RA_PRIO(1);
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       s[sub] = ra_zero16();
@@ -108,13 +112,14 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
       for (int ks = 0; ks < KS; ++ks)
         s[sub] = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s[sub]);
     }
+    RA_PRIO(0);
     float mx = -INFINITY, ce[KT / 32], be[KT / 32];
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);           // tile distances: rel0 - 31 .. rel0 + 31
       const int jl = j0 + 4 * lk;
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
-      ra_bias_mask<1>(s[sub], lut + (near ? jl - pi + p.R + RA_PAD : 0), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+      ra_bias_mask<1>(s[sub], lut + (near ? jl - pi + p.R + RA_PAD : 0), near, rel0 > 0 ? far_above : far_below,
                       j0 + 32 > kend || (p.causal && rel0 + 31 > 0), p.c, ce[sub], be[sub],
                       [&](int o) { return jl + o >= kend || (p.causal && jl + o > pi); });
       float x = s[sub][0];
@@ -152,8 +157,8 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
       }
     }
   }
-  if (i >= p.Lq) return;
   l += __shfl_xor(l, 32);
+  if (i >= p.Lq) return;
   const bool some = l != 0.f && i < nq;                   // rows behind the last query went along with their tile
   const float inv = some ? 1.0f / l : 0.f;
   if (!some) {
@@ -550,8 +555,8 @@ static int ra_fwd(RaParams& p, int few, void* stream) {
   }
   constexpr int NT = RaType<T>::NT, KT = NT == 3 && DP > 64 ? 32 : 64;
   const size_t lds = RaFwd<T, DP, KT>::bytes(p.R);
-  return ra_launch(rel_attn_fwd_kernel<T, DP, KT>, dim3((unsigned)((long)p.B * p.Hq * ((p.Lq + 127) / 128))), 256, lds,
-                   stream, p);
+  const long nqt = (p.Lq + 127) / 128, heads = (long)p.B * p.Hq;
+  return ra_launch(rel_attn_fwd_kernel<T, DP, KT>, dim3((unsigned)(heads * nqt)), 256, lds, stream, p);
 }
 
 extern "C" long occf_rel_attn_workspace(const int64_t* geom, int dtype) {

@@ -63,6 +63,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
   ra_fill_bias<T>(lut, p, h, tid, TH);
+  float far_below, far_above;
+  ra_far_bias<T>(p, h, far_below, far_above);
 
   const int i0 = qt * QW + wave * 32, i = i0 + li, pi = start + i;
   const bool live = i < nq;
@@ -143,15 +145,17 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= kend || (p.causal && rel0 > 31)) continue;
       f32x16 s = ra_zero16(), dp = dp_first;
+      RA_PRIO(1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_k, sub * 32, ks, li, lk), qf[ks], s);
         dp = ra_mm<NT>(ra_read_row<NT, DP, KT>(img_v, sub * 32, ks, li, lk), of[ks], dp);
       }
+      RA_PRIO(0);
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
       const int jl = j0 + 4 * lk;
       float ce, be;
-      ra_bias_mask<1>(s, lut + (near ? jl - pi + p.R + RA_PAD : 0), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+      ra_bias_mask<1>(s, lut + (near ? jl - pi + p.R + RA_PAD : 0), near, rel0 > 0 ? far_above : far_below,
                       j0 + 32 > kend || (p.causal && rel0 + 31 > 0), p.c, ce, be,
                       [&](int o) { return jl + o >= kend || (p.causal && jl + o > pi); });
       be -= lse;
@@ -162,6 +166,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
         ds[r] = pv[r] * dp[r];
         eps += ds[r];
       }
+      RA_PRIO(1);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const RaFrag<NT> df = ra_pack8<NT>(ds + s2 * 8), pf = ra_pack8<NT>(pv + s2 * 8);
@@ -172,6 +177,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
           if (PK) pk[dt] = ra_mm<NT>(kt_f, pf, pk[dt]);
         }
       }
+      RA_PRIO(0);
     }
   }
   eps += __shfl_xor(eps, 32);
@@ -278,6 +284,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     dk[dt] = ra_zero16();
     dv[dt] = ra_zero16();
   }
+  float far_below = 0.f, far_above = 0.f;                // the head's biases there
   float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
   RaTileRegs<T, DP, QT, TH> rq, ro;
   const long osl = (long)p.Hq * p.D;
@@ -339,6 +346,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     __syncthreads();
     if (step == t0 || at == 0) {
       ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
+      ra_far_bias<T>(p, hk * G + hg, far_below, far_above);
       if (NBUF == 2) __syncthreads();
     }
     if (NBUF == 1) {
@@ -364,15 +372,17 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
         s[4 * q] = x.x; s[4 * q + 1] = x.y; s[4 * q + 2] = x.z; s[4 * q + 3] = x.w;
         dp[4 * q] = y.x; dp[4 * q + 1] = y.y; dp[4 * q + 2] = y.z; dp[4 * q + 3] = y.w;
       }
+      RA_PRIO(1);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = ra_mm<NT>(ra_read_row<NT, DP, QT>(img_q, sub * 32, ks, li, lk), kf[ks], s);
         dp = ra_mm<NT>(ra_read_row<NT, DP, QT>(img_o, sub * 32, ks, li, lk), vf[ks], dp);
       }
+      RA_PRIO(0);
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
       const int pl = start + i0 + 4 * lk;                // position of row 0 of this lane
       float ce, be;
-      ra_bias_mask<-1>(s, lut + (near ? j - pl + p.R + RA_PAD : 32), near, lut[rel0 > 0 ? 2 * p.R + RA_PAD : RA_PAD],
+      ra_bias_mask<-1>(s, lut + (near ? j - pl + p.R + RA_PAD : 32), near, rel0 > 0 ? far_above : far_below,
                        j0 + 32 > nk || (p.causal && rel0 + 31 > 0), p.c, ce, be,
                        [&](int o) { return !live || (p.causal && j > pl + o); });
       float ds[16], pv[16];

@@ -63,6 +63,7 @@ class HipOps:
         self._mgp_reverse = 0
         self.use_fused_swin = os.environ.get("OCCF_FUSED_SWIN", "1") == "1"
         self.use_fused_mlp = os.environ.get("OCCF_FUSED_MLP", "1") == "1"
+        self._plans = {}             # checked argument layouts of the position operators (see _plan)
 
     # ------------------------------------------------------------------ plumbing
     def _stream(self):
@@ -1204,11 +1205,36 @@ class HipOps:
 
     def _launch_on(self, t, name, *args):
         """``_call`` with the stream of the tensors' own device, which need not be the current one"""
-        if t.is_cuda and t.device.index != torch.cuda.current_device():
+        if self.strict and t.device.index != torch.cuda.current_device():
             with torch.cuda.device(t.device):
                 self._call(name, *args, self._stream())
         else:
             self._call(name, *args, self._stream())
+
+    def _plan(self, check, tensors, *rest):
+        """``check(*tensors, *rest)`` -> (plan, tensors as the kernels take them), once per layout: shapes, strides, types and
+        devices of the tensors and the other arguments say everything the checks look at but the addresses, and a call on a
+        layout that was checked before, whose tensors go to the kernel as they are, takes the plan of then (25 us of checks
+        beside a kernel of 3 for a single token)."""
+        key = (check.__name__, rest, *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
+        plan = self._plans.get(key)
+        if plan is not None and self._direct(plan[0], tensors):
+            return plan, tensors
+        plan, taken = check(*tensors, *rest)
+        if all(x is y for x, y in zip(tensors, taken)):
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            self._plans[key] = plan
+        return plan, taken
+
+    @staticmethod
+    def _direct(align, tensors):
+        """do the first ``align[1]`` tensors' addresses divide by ``align[0]``"""
+        at = 0
+        for t in tensors[:align[1]]:
+            if t is not None:
+                at |= t.data_ptr()
+        return at % align[0] == 0
 
     @staticmethod
     def _heads(what, name, t, dtype, heads=None, dim=None):
@@ -1248,8 +1274,9 @@ class HipOps:
         return cos.contiguous(), sin.contiguous(), positions, 2 * half, cos.shape[0], A, dims[0], \
             (dims[0] + dims[1] if A > 1 else half), per_b
 
-    def _qk_norm_rope_args(self, what, q, k, q_weight, k_weight, cos, sin, positions, axis_dims, interleaved, grads=()):
-        dt = self._on_device(what, q, k, q_weight, k_weight, cos, sin, positions, *grads)
+    def _check_norm(self, q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out, axis_dims, interleaved, what):
+        grads = what != "qk_norm_rope"
+        dt = self._on_device(what, q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out)
         q = self._heads(what, "q", q, q.dtype)
         B, L, Hq, D = q.shape
         if D % 2 or D > 128:
@@ -1259,24 +1286,27 @@ class HipOps:
         for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
             if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype):
                 raise OccfError(f"{what}: {name} must be [{D}] of {q.dtype}")
-        strides = q.stride()[:3]
         if k is not None:
             k = self._heads(what, "k", k, q.dtype, dim=D)
             if k.shape[:2] != q.shape[:2]:
                 raise OccfError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} need the same batch and length")
-            strides = strides + k.stride()[:3]
-        else:
-            strides = strides + (0, 0, 0)
         cos, sin, positions, rot, rows, axes, c1, c2, per_b = self._rotation(what, q, cos, sin, positions, axis_dims)
-        w = [None if x is None else x.contiguous() for x in (q_weight, k_weight)]
+        q_weight, k_weight = (None if x is None else x.contiguous() for x in (q_weight, k_weight))
         if interleaved:                                                   # a pair is one load
             even = lambda t: t if t is None or (t.data_ptr() % (2 * t.element_size()) == 0 and
                                                 not any(s % 2 for s in t.stride()[:-1])) \
                 else t.clone(memory_format=torch.contiguous_format)
-            q, k, w = even(q), even(k), [even(x) for x in w]
-            strides = q.stride()[:3] + ((0, 0, 0) if k is None else k.stride()[:3])
+            q, k, q_weight, k_weight = even(q), even(k), even(q_weight), even(k_weight)
+        if grads:
+            for name, x, g in (("dq_out", q, dq_out), ("dk_out", k, dk_out)):
+                if (x is None) != (g is None) or (x is not None and (g.shape != x.shape or g.dtype != q.dtype)):
+                    raise OccfError(f"{what}: {name} must have the shape and type of its output")
+            dq_out, dk_out = (None if g is None else self._aligned(g.contiguous()) for g in (dq_out, dk_out))
+        strides = q.stride()[:3] + ((0, 0, 0) if k is None else k.stride()[:3])
         geom = (ctypes.c_int64 * 17)(B, L, Hq, 0 if k is None else k.shape[2], D, rot, rows, axes, c1, c2, per_b, *strides)
-        return dt, q, k, w, cos, sin, positions, geom
+        taken = (q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out)
+        # addresses: pairs of columns are one load, gradients are read 16 bytes at a time, else any
+        return ((16 if grads else 2 * q.element_size() if interleaved else 1, len(taken)), dt, geom), taken
 
     def qk_norm_rope(self, q, k, q_weight, k_weight, cos=None, sin=None, positions=None, eps=1e-6, axis_dims=None,
                      interleaved=False):
@@ -1286,34 +1316,36 @@ class HipOps:
         ``positions`` int32 [L] or [B, L] (default 0 .. L - 1), [.., L, axes] where ``axis_dims`` gives the table's columns of each
         axis.  A position outside the table makes the turned columns of its rows NaN.  cos None: the norm alone.
         fp32 or bf16 (arithmetic fp32, one rounding) -> new contiguous (q, k)."""
-        dt, q, k, w, cos, sin, positions, geom = self._qk_norm_rope_args("qk_norm_rope", q, k, q_weight, k_weight, cos, sin,
-                                                                        positions, axis_dims, interleaved)
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
-        self._launch_on(q, "occf_qk_norm_rope_fwd", P(q), P(k), P(w[0]), P(w[1]), P(cos), P(sin), P(positions), P(qo), P(ko),
-                        geom, float(eps), int(bool(interleaved)), dt)
+        axis_dims, interleaved = None if axis_dims is None else tuple(axis_dims), bool(interleaved)
+        (_, dt, geom), (q, k, qw, kw, cos, sin, positions, _, _) = self._plan(
+            self._check_norm, (q, k, q_weight, k_weight, cos, sin, positions, None, None), axis_dims, interleaved,
+            "qk_norm_rope")
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        ko = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+        P = self._address
+        self._launch_on(q, "occf_qk_norm_rope_fwd", P(q), P(k), P(qw), P(kw), P(cos), P(sin), P(positions), P(qo), P(ko),
+                        geom, float(eps), interleaved, dt)
         return qo, ko
 
     def qk_norm_rope_backward(self, q, k, q_weight, k_weight, dq_out, dk_out, cos=None, sin=None, positions=None, eps=1e-6,
                               axis_dims=None, interleaved=False):
         """-> (dq, dk, dq_weight, dk_weight) for the gradients dq_out, dk_out of ``qk_norm_rope``'s outputs"""
-        what = "qk_norm_rope_backward"
-        dt, q, k, w, cos, sin, positions, geom = self._qk_norm_rope_args(what, q, k, q_weight, k_weight, cos, sin, positions,
-                                                                        axis_dims, interleaved, (dq_out, dk_out))
-        for name, x, g in (("dq_out", q, dq_out), ("dk_out", k, dk_out)):
-            if (x is None) != (g is None) or (x is not None and (g.shape != x.shape or g.dtype != q.dtype)):
-                raise OccfError(f"{what}: {name} must have the shape and type of its output")
-        dq_out, dk_out = self._aligned(dq_out.contiguous()), None if k is None else self._aligned(dk_out.contiguous())
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dqw = torch.empty_like(w[0])
-        dkw = None if k is None else torch.empty_like(w[1])
+        axis_dims, interleaved = None if axis_dims is None else tuple(axis_dims), bool(interleaved)
+        (_, dt, geom), (q, k, qw, kw, cos, sin, positions, dq_out, dk_out) = self._plan(
+            self._check_norm, (q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out), axis_dims, interleaved,
+            "qk_norm_rope_backward")
+        dq, dqw, dk, dkw = torch.empty_like(dq_out), torch.empty_like(qw), None, None
+        if k is not None:
+            dk, dkw = torch.empty_like(dk_out), torch.empty_like(kw)
         ws = self._ws(self.lib.occf_qk_norm_rope_bwd_workspace(q.shape[3]), q.device)
-        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
-        self._launch_on(q, "occf_qk_norm_rope_bwd", P(q), P(k), P(w[0]), P(w[1]), P(cos), P(sin), P(positions), P(dq_out),
-                        P(dk_out), P(dq), P(dk), P(dqw), P(dkw), P(ws), geom, float(eps), int(bool(interleaved)), dt)
+        P = self._address
+        self._launch_on(q, "occf_qk_norm_rope_bwd", P(q), P(k), P(qw), P(kw), P(cos), P(sin), P(positions), P(dq_out),
+                        P(dk_out), P(dq), P(dk), P(dqw), P(dkw), P(ws), geom, float(eps), interleaved, dt)
         return dq, dk, dqw, dkw
+
+    @staticmethod
+    def _address(t):
+        return None if t is None else t.data_ptr()
 
     @staticmethod
     def _aligned(t):
@@ -1324,8 +1356,9 @@ class HipOps:
             return t.clone(memory_format=torch.contiguous_format)
         return t
 
-    def _rel_attention_args(self, what, q, k, v, table, buckets, scale, causal, lens, grads=()):
-        dt = self._on_device(what, q, k, v, table, buckets.lut, *lens, *grads)
+    def _check_rel_attention(self, q, k, v, out, dout, table, lut, q_lens, k_lens, q_start, lse, nb, radius, scale, causal,
+                             what):
+        dt = self._on_device(what, q, k, v, table, lut, q_lens, k_lens, q_start, out, dout, lse)
         q = self._heads(what, "q", q, q.dtype)
         B, Lq, Hq, D = q.shape
         k, v = self._heads(what, "k", k, q.dtype, dim=D), self._heads(what, "v", v, q.dtype, dim=D)
@@ -1335,19 +1368,29 @@ class HipOps:
                             "divide the query heads")
         if D % 8 or D > 128:
             raise OccfError(f"{what}: head dim {D} must be a multiple of 8, at most 128")
-        if tuple(table.shape) != (buckets.num_buckets, Hq) or table.dtype != q.dtype:
-            raise OccfError(f"{what}: table must be [{buckets.num_buckets}, {Hq}] of {q.dtype}, got {tuple(table.shape)} of "
-                            f"{table.dtype}")
-        for name, t in zip(("q_lens", "k_lens", "q_start"), lens):
+        if tuple(table.shape) != (nb, Hq) or table.dtype != q.dtype:
+            raise OccfError(f"{what}: table must be [{nb}, {Hq}] of {q.dtype}, got {tuple(table.shape)} of {table.dtype}")
+        for name, t in (("q_lens", q_lens), ("k_lens", k_lens), ("q_start", q_start)):
             if t is not None and (tuple(t.shape) != (B,) or t.dtype != self.i32):
                 raise OccfError(f"{what}: {name} must be int32 [{B}]")
-        scale = float(D) ** -0.5 if scale is None else float(scale)
+        scale = float(D) ** -0.5 if scale is None else scale
         if not 0.0 < scale < float("inf"):
             raise OccfError(f"{what}: scale {scale} must be positive")
         q, k, v = self._aligned(q), self._aligned(k), self._aligned(v)
-        geom = (ctypes.c_int64 * 17)(B, Lq, Lk, Hq, Hk, D, buckets.num_buckets, buckets.radius, *q.stride()[:3],
-                                     *k.stride()[:3], *v.stride()[:3])
-        return dt, q, k, v, table.contiguous(), tuple(None if t is None else t.contiguous() for t in lens), scale, geom
+        if lse is not None:
+            for name, t in (("out", out), ("dout", dout)):
+                if t is None or t.shape != q.shape or t.dtype != q.dtype:
+                    raise OccfError(f"{what}: {name} must have the shape and type of q")
+            if tuple(lse.shape) != (B, Hq, Lq) or lse.dtype != self.f32:
+                raise OccfError(f"{what}: lse must be fp32 [{B}, {Hq}, {Lq}]")
+            out, dout, lse = self._aligned(out.contiguous()), self._aligned(dout.contiguous()), lse.contiguous()
+        geom = (ctypes.c_int64 * 17)(B, Lq, Lk, Hq, Hk, D, nb, radius, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
+        need = self.lib.occf_rel_attn_workspace(geom, dt) if lse is None else \
+            self.lib.occf_rel_attn_bwd_workspace(geom, causal, dt)
+        if need < 0:
+            raise OccfError(f"{what}: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        lens = (None if t is None else t.contiguous() for t in (q_lens, k_lens, q_start))
+        return ((16, 5), dt, geom, scale, need), (q, k, v, out, dout, table.contiguous(), lut, *lens, lse)
 
     def rel_attention(self, q, k, v, table, buckets, scale=None, causal=False, q_lens=None, k_lens=None, q_start=None,
                       return_lse=False):
@@ -1357,48 +1400,35 @@ class HipOps:
         j <= p_i; other rows, and rows that see no key, are zeros.  A table entry at or below -1e30 takes its bucket out.
         One query of a sequence that grows: q_start = k_lens - 1.  fp32 or bf16 -> [B, Lq, Hq, D]; with ``return_lse`` also the
         rows' base-2 logarithms of the sum of exponentials, fp32 [B, Hq, Lq], for ``rel_attention_backward``.
-        bf16: probabilities are rounded to bf16 before the product with v (their sum is not)."""
-        dt, q, k, v, table, lens, scale, geom = self._rel_attention_args("rel_attention", q, k, v, table, buckets, scale, causal,
-                                                                        (q_lens, k_lens, q_start))
-        B, Lq, Hq, _ = q.shape
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty((B, Hq, Lq), dtype=self.f32, device=q.device) if return_lse else None
-        need = self.lib.occf_rel_attn_workspace(geom, dt)
-        if need < 0:
-            raise OccfError(f"rel_attention: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        bf16: probabilities are rounded to bf16 before their sum and the product with v."""
+        causal = bool(causal)
+        (_, dt, geom, scale, need), (q, k, v, _, _, table, lut, q_lens, k_lens, q_start, _) = self._plan(
+            self._check_rel_attention, (q, k, v, None, None, table, buckets.lut, q_lens, k_lens, q_start, None),
+            buckets.num_buckets, buckets.radius, None if scale is None else float(scale), causal, "rel_attention")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=self.f32, device=q.device) if return_lse else None
         ws = torch.empty((need,), dtype=self.f32, device=q.device) if need else None
-        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
-        self._launch_on(q, "occf_rel_attn_fwd", P(q), P(k), P(v), P(table), P(buckets.lut), P(lens[0]), P(lens[1]), P(lens[2]),
-                        P(out), P(lse), P(ws), need, geom, scale, int(bool(causal)), dt)
+        P = self._address
+        self._launch_on(q, "occf_rel_attn_fwd", P(q), P(k), P(v), P(table), P(lut), P(q_lens), P(k_lens), P(q_start), P(out),
+                        P(lse), P(ws), need, geom, scale, causal, dt)
         return (out, lse) if return_lse else out
 
     def rel_attention_backward(self, q, k, v, table, buckets, out, lse, dout, scale=None, causal=False, q_lens=None,
                                k_lens=None, q_start=None):
         """-> (dq, dk, dv, dtable) for ``rel_attention``'s out, lse and the gradient dout of out; rows that do not count get
-        zeros.  bf16: P and dS are rounded to bf16 before their products, dtable's sums are not; the rows' <dout, out> come
-        from the rounded out."""
-        what = "rel_attention_backward"
-        dt, q, k, v, table, lens, scale, geom = self._rel_attention_args(what, q, k, v, table, buckets, scale, causal,
-                                                                        (q_lens, k_lens, q_start), (out, lse, dout))
-        B, Lq, Hq, _ = q.shape
-        for name, t in (("out", out), ("dout", dout)):
-            if t.shape != q.shape or t.dtype != q.dtype:
-                raise OccfError(f"{what}: {name} must have the shape and type of q")
-        if tuple(lse.shape) != (B, Hq, Lq) or lse.dtype != self.f32:
-            raise OccfError(f"{what}: lse must be fp32 [{B}, {Hq}, {Lq}]")
-        out, dout, lse = self._aligned(out.contiguous()), self._aligned(dout.contiguous()), lse.contiguous()
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dtable = torch.empty_like(table)
-        need = self.lib.occf_rel_attn_bwd_workspace(geom, int(bool(causal)), dt)
-        if need < 0:
-            raise OccfError(f"{what}: sizes outside the kernels' limits: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        zeros.  bf16: P and dS are rounded to bf16 before their products, dtable's sums are not."""
+        causal = bool(causal)
+        (_, dt, geom, scale, need), (q, k, v, out, dout, table, lut, q_lens, k_lens, q_start, lse) = self._plan(
+            self._check_rel_attention, (q, k, v, out, dout, table, buckets.lut, q_lens, k_lens, q_start, lse),
+            buckets.num_buckets, buckets.radius, None if scale is None else float(scale), causal,
+            "rel_attention_backward")
+        dq, dtable = torch.empty_like(dout), torch.empty_like(table)
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         ws = torch.empty((need,), dtype=self.f32, device=q.device)
-        P = lambda t: ctypes.c_void_p(0 if t is None else t.data_ptr())
-        self._launch_on(q, "occf_rel_attn_bwd", P(q), P(k), P(v), P(table), P(buckets.lut), P(lens[0]), P(lens[1]), P(lens[2]),
-                        P(out), P(lse), P(dout), P(dq), P(dk), P(dv), P(dtable), P(ws), need, geom, scale,
-                        int(bool(causal)), dt)
+        P = self._address
+        self._launch_on(q, "occf_rel_attn_bwd", P(q), P(k), P(v), P(table), P(lut), P(q_lens), P(k_lens), P(q_start), P(out),
+                        P(lse), P(dout), P(dq), P(dk), P(dv), P(dtable), P(ws), need, geom, scale, causal, dt)
         return dq, dk, dv, dtable
 
     # ------------------------------------------------------------------ img_inputs producer (csrc/pipeline.hip)

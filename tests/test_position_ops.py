@@ -404,6 +404,18 @@ def test_rel_attention_many_rows(be, D, causal, dtype):
     _check_attention(be, (13, 40, 70, 10, 5, D, causal, 8, 12, not causal, rows), dtype, backward=False)
 
 
+@pytest.mark.parametrize("Lq", [260, 129])
+def test_rel_attention_causal_tiles(be, Lq):
+    """causal, several tiles of 128 queries and more heads than one round of the workgroups' order takes"""
+    heads = 256
+    case = (1, Lq, Lq, heads, heads // 8, 8, True, 8, 12, False, [(Lq, Lq - 5, 3)])
+    q, k, v, table, plan, lens, _ = _attn_inputs(case, torch.bfloat16)
+    ref = _attn_ref(q, k, v, table, plan, True, 8 ** -0.5, *lens, None, torch.bfloat16)
+    out = be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), causal=True, q_lens=be.to(lens[0]),
+                               k_lens=be.to(lens[1]), q_start=be.to(lens[2]))
+    _within(out, *ref["out"], "out")
+
+
 def test_rel_attention_taken_out_buckets(be):
     """a table entry at the type's lowest value or -inf takes its bucket out, and a row left with nothing is zeros"""
     for dtype in (torch.float32, torch.bfloat16):
