@@ -9,7 +9,7 @@
 //   rel_attn_dkv_kernel  a wave owns 32 keys (lane = key) and walks the queries of every head that shares them:
 //                        S = Q K^T, dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS, and the distances' sums of dS
 // The scores are formed twice: 7 products instead of 5, where a single pass would have to add dQ up across workgroups.
-// -delta (and -lse / c where it is a row's, not a lane's) is the accumulators' first value: no instruction a score.
+// -delta (in the second kernel, for bf16, -lse / c too) is the accumulators' first value: no instruction a score.
 //
 // delta: a row of dS sums to zero, but <dO, O> of an O rounded to bf16 (whose P was rounded too) is off by a few 2^-9, and the
 // bias' gradient, sums of dS that nearly cancel, shows it (3.5e-3 of error where its own rounding is 1.7e-3).  The row sums of
@@ -228,6 +228,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   const RaParams& p = g.a;
   typedef RaDkv<T, DP, QT, NW> L;
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, KW = NW * 32, NBUF = L::NBUF;
+  // -lse / c as the scores' first value rounds every partial sum at its size (12 / c = 40 at 1000 keys): 1e-6 of P, not for fp32
+  constexpr bool LSE_FIRST = NT == 1;
   OCCF_DYN_SMEM(smem);
   float* tiles = (float*)(smem + NBUF * L::tile);
   float* lut = tiles + NW * RA_DTILE;
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     if (tid < QT) {
       // rows that do not count or see no key: P = 0
       const bool row = nrow + tid < nend;
-      s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : -nlse / p.c;
+      s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : LSE_FIRST ? -nlse / p.c : -nlse;
       float x = ndelta[0];
 #pragma unroll
       for (int s = 1; s < RA_QSPLIT; ++s)
@@ -365,11 +367,19 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       const int i0 = r0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= nk || i0 >= nq || (p.causal && rel0 > 31)) continue;      // wave-uniform
       f32x16 s, dp;
+      float off[LSE_FIRST ? 1 : 16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float4 x = *(const float4*)(s_lse + sub * 32 + 8 * q + 4 * lk);
         const float4 y = *(const float4*)(s_delta + sub * 32 + 8 * q + 4 * lk);
         s[4 * q] = x.x; s[4 * q + 1] = x.y; s[4 * q + 2] = x.z; s[4 * q + 3] = x.w;
+        if (!LSE_FIRST) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            off[LSE_FIRST ? 0 : 4 * q + e] = s[4 * q + e];
+            s[4 * q + e] = 0.f;
+          }
+        }
         dp[4 * q] = y.x; dp[4 * q + 1] = y.y; dp[4 * q + 2] = y.z; dp[4 * q + 3] = y.w;
       }
       RA_PRIO(1);
@@ -388,7 +398,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       float ds[16], pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        pv[r] = ra_exp2(fmaf(s[r], ce, be));
+        pv[r] = ra_exp2(fmaf(s[r], ce, LSE_FIRST ? be : be + off[LSE_FIRST ? 0 : r]));
         ds[r] = pv[r] * dp[r];
       }
       if (near) {
