@@ -20,14 +20,12 @@
 #include "rel_attn.h"
 #include "../../include/occformer_hip.h"
 
-// Half a 32 x 32 tile whose diagonals are summed: rows of 72 floats of which the last 40 stay zero, as do 32 before the first,
-// so that a lane's walk down its diagonal needs no test (16 reads at constant offsets).  A whole tile would leave room for one
-// workgroup a compute unit instead of two (523 instead of 409 us at 2 x 4096 causal rows, 16 heads of 64).
-#define RA_DLD 72
-#define RA_DFRONT 32
-#define RA_DTILE (RA_DFRONT + 16 * RA_DLD)
-
-#define RA_QSPLIT 8             // most parts of the keys that a query's walk is cut into
+// The 32 x 32 tile whose diagonals are summed: rows of 64 floats of which the last 32 stay zero, as do 32 before the first, so
+// that a lane's walk down its diagonal needs no test (32 reads at constant offsets).  fp32 with more than 64 columns has room for
+// half a tile beside its operand images, and sums it in two goes.
+template <class T, int DP> struct RaDiag {
+  static constexpr int ROWS = RaType<T>::NT == 3 && DP > 64 ? 16 : 32, LD = 64, FRONT = 32, floats = FRONT + ROWS * LD;
+};
 
 struct RaBwd {
   RaParams a;
@@ -111,7 +109,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   rk.place(p.ksl, p.D, tid);
   rv.place(p.vsl, p.D, tid);
   const int ntile = (kend + KT - 1) / KT;
-  const int t0 = (int)((long)ntile * split / g.qsplit), t1 = (int)((long)ntile * (split + 1) / g.qsplit);
+  const int t0 = (int)((unsigned)(ntile * split) / (unsigned)g.qsplit), t1 = (int)((unsigned)(ntile * (split + 1)) / (unsigned)g.qsplit);
   const auto load = [&](int k0) {
     rk.load(kb + k0 * p.ksl, p.ksl, kend - k0, p.D);
     rv.load(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
@@ -140,7 +138,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     const char* img_k = smem + (NBUF == 2 ? (kt - t0) & 1 : 0) * RaDq<T, DP, KT>::tile;
     const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
     if (i0 >= nq) continue;                              // wave-uniform
-#pragma unroll
+#pragma unroll 1
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int j0 = k0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= kend || (p.causal && rel0 > 31)) continue;
@@ -182,9 +180,10 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   }
   eps += __shfl_xor(eps, 32);
   if (i >= p.Lq) return;
-  // one part: the corrected delta; several: the parts' sums, delta among the first one's
-  if (lk == 0) p.delta[(long)split * p.B * p.Hq * p.Lq + stat] = split == 0 ? delta + eps : eps;
-  if (lk == 0 && g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;
+  if (lk == 0) {
+    if (split == 0) p.delta[stat] = g.qsplit > 1 ? delta : delta + eps;
+    if (g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;      // rel_attn_finish_kernel adds these to delta
+  }
   const long part = (long)split * p.B * p.Lq * p.Hq * p.D + orow;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -208,19 +207,15 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
     }
 }
 
-// one statistic of a row: array [parts][B][Hq][Lq], byte offset `at` within the batch entry; `ok` false: 0
-__device__ __forceinline__ float ra_load_stat(const float* x, const RaParams& p, int b, int part, uint32_t at, bool ok) {
-  const long n = (long)p.Hq * p.Lq;
-  const occf_bbuf buf = occf_make_bbuf(x + ((long)part * p.B + b) * n, (uint32_t)n * 4u);
-  return ra_buf4(buf, ok ? at : OCCF_BUF_OOB);
-}
-
 template <class T, int DP, int QT, int NW>
 struct RaDkv {
   static constexpr int images = 2 * RaType<T>::NT * RaRow<DP>::bytes(QT);                // Q and dO
   static constexpr int tile = images + 2 * QT * 4;                                       // and the rows' statistics
   static constexpr int NBUF = tile <= 20 * 1024 ? 2 : 1;                                 // (see rel_attn_fwd_kernel)
-  static size_t bytes(int R) { return NBUF * tile + 4 * ((NW + 1) * (2 * (size_t)R + 1 + 2 * RA_PAD) + NW * RA_DTILE); }
+  static size_t bytes(int R) {
+    const size_t nl = 2 * (size_t)R + 1 + 2 * RA_PAD;
+    return NBUF * tile + 4 * ((NW + 1) * nl + NW * RaDiag<T, DP>::floats) + nl;
+  }
 };
 
 template <class T, int DP, int QT, int NW>
@@ -232,13 +227,13 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   constexpr bool LSE_FIRST = NT == 1;
   OCCF_DYN_SMEM(smem);
   float* tiles = (float*)(smem + NBUF * L::tile);
-  float* lut = tiles + NW * RA_DTILE;
+  float* lut = tiles + NW * RaDiag<T, DP>::floats;
   const int nl = 2 * p.R + 1 + 2 * RA_PAD;
   float* sums = lut + nl;                                // [NW][nl] sums of dS by distance
   const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & 31, lk = lane >> 5;
   float* dsum = sums + wave * nl;
-  float* tile = tiles + wave * RA_DTILE + RA_DFRONT;
-  for (int t = tid; t < NW * RA_DTILE; t += TH) tiles[t] = 0.f;
+  float* tile = tiles + wave * RaDiag<T, DP>::floats + RaDiag<T, DP>::FRONT;
+  uint8_t* ids = (uint8_t*)(sums + NW * nl);             // bucket of every distance
 
   const int nkt = (p.Lk + KW - 1) / KW, G = p.Hq / p.Hk;
   int kt, bh;
@@ -270,7 +265,14 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   }
   const int ntile = kt * KW >= nk || first >= nq ? 0 : (nq - first + QT - 1) / QT;
   // steps: the query tiles of every head of the group, in order; this workgroup's share of them
-  const int t0 = (int)((long)ntile * G * split / g.ksplit), t1 = (int)((long)ntile * G * (split + 1) / g.ksplit);
+  const unsigned steps = (unsigned)(ntile * G);
+  const int t0 = (int)(steps * split / (unsigned)g.ksplit), t1 = (int)(steps * (split + 1) / (unsigned)g.ksplit);
+  float far_below = 0.f, far_above = 0.f;                // the head's biases at distances <= -R and >= R
+  const int hg0 = t0 < t1 ? t0 / ntile : 0;
+  ra_fill_bias<T>(lut, p, hk * G + hg0, tid, TH);
+  ra_far_bias<T>(p, hk * G + hg0, far_below, far_above);
+  for (int t = tid; t < nl; t += TH) ids[t] = (uint8_t)occf_clampi(p.lut[occf_clampi(t - RA_PAD, 2 * p.R)], p.nb - 1);
+  for (int t = tid; t < NW * RaDiag<T, DP>::floats / 4; t += TH) ra_store4(tiles + 4 * t, 0.f, 0.f, 0.f, 0.f);
   float* tab = g.tab_part + ((((long)b * p.Hk + hk) * g.ksplit + split) * nkt + kt) * G * p.nb;       // [G][nb]
 
   for (int t = tid; t < NW * nl; t += TH) sums[t] = 0.f;
@@ -286,7 +288,6 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     dk[dt] = ra_zero16();
     dv[dt] = ra_zero16();
   }
-  float far_below = 0.f, far_above = 0.f;                // the head's biases there
   float below = 0.f, above = 0.f;                        // sums of dS at distances <= -R and >= R
   RaTileRegs<T, DP, QT, TH> rq, ro;
   const long osl = (long)p.Hq * p.D;
@@ -294,8 +295,11 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   ro.place(osl, p.D, tid);
   // the next tile's rows, and on QT lanes their statistics, all looked at only when the tile is stored: a value that is used
   // where it is loaded would make the workgroup wait for it in every step
-  float nlse = 0.f, ndelta[RA_QSPLIT];
-  int hg = t0 < t1 ? t0 / ntile : 0, at = t0 - hg * ntile;               // head of the group and query tile of a step
+  float nlse = 0.f, ndelta = 0.f;
+  const long nstat = (long)p.Hq * p.Lq;
+  const occf_bbuf lse_buf = occf_make_bbuf(p.lse + b * nstat, (uint32_t)nstat * 4u);
+  const occf_bbuf delta_buf = occf_make_bbuf(p.delta + b * nstat, (uint32_t)nstat * 4u);
+  int hg = hg0, at = t0 - hg * ntile;                                    // head of the group and query tile of a step
   int lstep = t0, lhg = hg, lat = at;                                    // ... of the next load
   int nrow = 0, nend = 0;                                                // the loaded tile's first query, and behind its last
   const auto load = [&]() {
@@ -305,11 +309,9 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     nend = more ? nq : 0;
     rq.load((const T*)p.q + (long)b * p.qsb + (long)h * p.qsh + r0 * p.qsl, p.qsl, nend - r0, p.D);
     ro.load((const T*)p.dout + ((long)b * p.Lq * p.Hq + h) * p.D + r0 * osl, osl, nend - r0, p.D);
-    const uint32_t stat = ((uint32_t)h * (uint32_t)p.Lq + (uint32_t)(r0 + tid)) * 4u;
-    nlse = ra_load_stat(p.lse, p, b, 0, stat, tid < QT && r0 + tid < nend);
-#pragma unroll
-    for (int s = 0; s < RA_QSPLIT; ++s)
-      if (s < g.qsplit) ndelta[s] = ra_load_stat(p.delta, p, b, s, stat, tid < QT && r0 + tid < nend);
+    const uint32_t stat = tid < QT && r0 + tid < nend ? ((uint32_t)h * (uint32_t)p.Lq + (uint32_t)(r0 + tid)) * 4u : OCCF_BUF_OOB;
+    nlse = ra_buf4(lse_buf, stat);
+    ndelta = ra_buf4(delta_buf, stat);
     ++lstep;
     if (++lat == ntile) {
       lat = 0;
@@ -326,11 +328,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       // rows that do not count or see no key: P = 0
       const bool row = nrow + tid < nend;
       s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : LSE_FIRST ? -nlse / p.c : -nlse;
-      float x = ndelta[0];
-#pragma unroll
-      for (int s = 1; s < RA_QSPLIT; ++s)
-        if (s < g.qsplit) x += ndelta[s];
-      s_delta[tid] = row ? -x : 0.f;
+      s_delta[tid] = -ndelta;
     }
   };
   load();
@@ -346,7 +344,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     }
     const int r0 = first + at * QT;
     __syncthreads();
-    if (step == t0 || at == 0) {
+    if (step > t0 && at == 0) {
       ra_fill_bias<T>(lut, p, hk * G + hg, tid, TH);
       ra_far_bias<T>(p, hk * G + hg, far_below, far_above);
       if (NBUF == 2) __syncthreads();
@@ -362,7 +360,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     const char* img_q = smem + (NBUF == 2 ? (step - t0) & 1 : 0) * L::tile;
     const char* img_o = img_q + NT * RaRow<DP>::bytes(QT);
     const float *s_lse = (const float*)(img_q + L::images), *s_delta = s_lse + QT;
-#pragma unroll
+#pragma unroll 1
     for (int sub = 0; sub < QT / 32; ++sub) {
       const int i0 = r0 + sub * 32, rel0 = j0 - (start + i0);
       if (j0 >= nk || i0 >= nq || (p.causal && rel0 > 31)) continue;      // wave-uniform
@@ -403,16 +401,17 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       }
       if (near) {
         // sums along the diagonals: lane e adds the pairs at distance rel0 + e - 31 (63 of them), in LDS of the wave's own
+        constexpr int DR = RaDiag<T, DP>::ROWS, DL = RaDiag<T, DP>::LD;
         float y[2] = {0.f, 0.f};
         const float* dg = tile + lane - 31;
 #pragma unroll
-        for (int hv = 0; hv < 2; ++hv) {
+        for (int hv = 0; hv < 32 / DR; ++hv) {
           RA_WAVE_SYNC();
 #pragma unroll
-          for (int r = 0; r < 8; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * RA_DLD + li] = ds[8 * hv + r];
+          for (int r = 0; r < DR / 2; ++r) tile[((r & 3) + 8 * (r >> 2) + 4 * lk) * DL + li] = ds[DR / 2 * hv + r];
           RA_WAVE_SYNC();
 #pragma unroll
-          for (int q = 0; q < 16; ++q) y[q & 1] += dg[q * (RA_DLD + 1) + 16 * hv];
+          for (int q = 0; q < DR; ++q) y[q & 1] += dg[q * (DL + 1) + DR * hv];
         }
         const float x = y[0] + y[1];
         if (lane < 63) dsum[rel0 + lane - 31 + p.R + RA_PAD] += x;
@@ -463,8 +462,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       const int tl = TH / nb2, bk = tid / tl, r = tid % tl;
       float x = 0.f;
       if (bk < p.nb)
-        for (int t = r; t < nl; t += tl)
-          if (occf_clampi(p.lut[occf_clampi(t - RA_PAD, 2 * p.R)], p.nb - 1) == bk) x += sums[t];
+#pragma unroll 4
+        for (int t = r; t < nl; t += tl) x += ids[t] == bk ? sums[t] : 0.f;
       for (int mm = 1; mm < tl; mm <<= 1) x += __shfl_xor(x, mm);
       if (bk < p.nb && r == 0) tab[hg * p.nb + bk] = x;
       __syncthreads();
@@ -495,14 +494,14 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     }
 }
 
-// The parts in order: the first Hq workgroups make the bias' gradient, then dq and then dk, dv where their walks were cut
-// (four columns a thread).
+// The parts in order.  Behind the first kernel, where its walk was cut: dq (four columns a thread), and a row's first thread
+// completes its delta.  Behind the second: the bias' gradient on Hq workgroups, then dk and dv where that walk was cut.
 template <class T>
-__global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int dq_blocks) {
+__global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int dq) {
   const RaParams& p = g.a;
   const int tid = threadIdx.x;
   int blk = blockIdx.x;
-  if (blk < p.Hq) {
+  if (!dq && blk < p.Hq) {
     __shared__ float acc[256];
     const int G = p.Hq / p.Hk, hk = blk / G, hg = blk % G;
     int nb2 = 1;
@@ -527,9 +526,8 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
     }
     return;
   }
-  blk -= p.Hq;
-  const bool dq = blk < dq_blocks;
-  const long at = ((long)(dq ? blk : blk - dq_blocks) * 256 + tid) * 4;
+  if (!dq) blk -= p.Hq;
+  const long at = ((long)blk * 256 + tid) * 4;
   const long n = dq ? (long)p.B * p.Lq * p.Hq * p.D : (long)p.B * p.Lk * p.Hk * p.D;
   if (at >= n) return;
   const int splits = dq ? g.qsplit : g.ksplit;
@@ -545,16 +543,15 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
     }
   }
   if (dq) {
+    const long row = at / p.D;                           // (b Lq + i) Hq + h
+    const int h = (int)(row % p.Hq);
+    const long bi = row / p.Hq;
+    const long stat = (bi / p.Lq * p.Hq + h) * p.Lq + bi % p.Lq;
     float eps = 0.f;
-    if (second) {
-      const long row = at / p.D;                         // (b Lq + i) Hq + h
-      const int h = (int)(row % p.Hq);
-      const long bi = row / p.Hq;
-      const long stat = (bi / p.Lq * p.Hq + h) * p.Lq + bi % p.Lq;
-      for (int s = 0; s < splits; ++s) eps += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
-    }
+    for (int s = 0; s < splits; ++s) eps += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
+    if (at == row * p.D) p.delta[stat] += eps;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = fmaf(-eps, y[e], x[e]) * p.scale;
+    for (int e = 0; e < 4; ++e) x[e] = (second ? fmaf(-eps, y[e], x[e]) : x[e]) * p.scale;
     ra_store4((T*)p.dq + at, x[0], x[1], x[2], x[3]);
   } else {
     ra_store4((T*)p.dk + at, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
@@ -570,8 +567,8 @@ static void ra_bwd_plan(const int64_t* g, int causal, int& qsplit, int& ksplit) 
   const long wq = B * Hq * ((Lq + 127) / 128), wk = B * Hk * ((Lk + 127) / 128);
   const long mq = (Lk + 127) / 128, mk = (Hq / Hk) * ((Lq + 127) / 128);
   const auto cut = [](long want, long most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
-  qsplit = cut(cut(512 / wq, mq), RA_QSPLIT);
-  ksplit = cut(cut(((causal ? 1024 : 512) + wk / 2) / wk, mk), 16);
+  qsplit = cut(cut(512 / wq, mq), 8);
+  ksplit = cut(cut((causal ? 1024 : 512) / wk, mk), 16);
 }
 
 struct RaBwdSizes { long delta, eps, dq, dk, tab; };
@@ -579,8 +576,8 @@ static RaBwdSizes ra_bwd_sizes(const int64_t* g, int qsplit, int ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6];
   RaBwdSizes s;
   const auto up = [](long n) { return (n + 63) / 64 * 64; };             // parts start on 256 bytes
-  s.delta = up(B * Hq * Lq * qsplit);
-  s.eps = qsplit > 1 ? s.delta : 0;
+  s.delta = up(B * Hq * Lq);
+  s.eps = qsplit > 1 ? up(B * Hq * Lq * qsplit) : 0;
   s.dq = qsplit > 1 ? up(B * Lq * Hq * D * qsplit) : 0;
   s.dk = ksplit > 1 ? up(B * Lk * Hk * D * ksplit) : 0;
   s.tab = up(B * Hq * ksplit * ((Lk + 127) / 128) * nb);
@@ -595,14 +592,18 @@ static int ra_bwd(const RaBwd& g, void* stream) {
   int rc = ra_launch(rel_attn_dq_kernel<T, DP, KT, NW>, dim3((unsigned)(p.B * p.Hq * nqt * g.qsplit)), NW * 64,
                      RaDq<T, DP, KT>::bytes(p.R), stream, g);
   if (rc) return rc;
+  const auto blocks = [](long n) { return (unsigned)((n / 4 + 255) / 256); };
+  if (g.qsplit > 1) {
+    hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(blocks((long)p.B * p.Lq * p.Hq * p.D)), dim3(256), 0, (hipStream_t)stream,
+                       g, (int)nkt, 1);
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
   rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW>, dim3((unsigned)(p.B * p.Hk * nkt * g.ksplit)), NW * 64,
                  RaDkv<T, DP, QT, NW>::bytes(p.R), stream, g);
   if (rc) return rc;
-  const auto blocks = [&](long n) { return (n / 4 + 255) / 256; };
-  const long dq = g.qsplit > 1 ? blocks((long)p.B * p.Lq * p.Hq * p.D) : 0;
-  const long dk = g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0;
-  hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3((unsigned)(p.Hq + dq + dk)), dim3(256), 0, (hipStream_t)stream, g, (int)nkt,
-                     (int)dq);
+  hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(p.Hq + (g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0)), dim3(256), 0,
+                     (hipStream_t)stream, g, (int)nkt, 0);
   OCCF_LAUNCH_CHECK();
 }
 
