@@ -416,6 +416,48 @@ def test_rel_attention_causal_tiles(be, Lq):
     _within(out, *ref["out"], "out")
 
 
+# key lengths of the sequences; None: all keys of all
+SINGLE = [(2, 700, 1, 1, 32, None), (3, 700, 4, 2, 24, [700, 0, 129]), (5, 513, 17, 1, 64, [1, 127, 128, 513, 400]),
+          (70, 300, 2, 2, 8, [(37 * b) % 301 for b in range(70)]), (2, 260, 32, 1, 128, [260, 31])]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", SINGLE)
+def test_rel_attention_single_queries(be, case, dtype):
+    """one query a sequence against its keys so far: 16 and 32 rows a key head, walks cut by the longest sequence and by every
+    sequence's own length, more sequences than a wave has lanes"""
+    B, Lk, G, Hk, D, lens = case
+    n = lens or [Lk] * B
+    rows = [(1, m, m - 1) for m in n]
+    _check_attention(be, (B, 1, Lk, G * Hk, Hk, D, True, 8, 40, False, rows), dtype, backward=False)
+    if lens is None:
+        q, k, v, table, plan, (_, _, start), _ = _attn_inputs((B, 1, Lk, G * Hk, Hk, D, True, 8, 40, False, rows), dtype)
+        a = be.to(q, k, v, table)
+        want = be.ops.rel_attention(*a, _plan_on(be, plan), causal=True, q_start=be.to(start))
+        lens = be.to(torch.tensor(n, dtype=torch.int32))
+        got = be.ops.rel_attention(*a, _plan_on(be, plan), causal=True, q_start=be.to(start), k_lens=lens)
+        # the same keys in other parts: as in test_prompt_then_single_tokens
+        tol = (3 * BF if dtype == torch.bfloat16 else (4 * Lk + 8 * D) * U) * float(v.abs().amax())
+        assert float((want - got).abs().max()) <= tol
+
+
+def test_rel_attention_lengths_out_of_range(be):
+    """lengths beyond the tensors count as all of it, negative ones as none; positions far outside stay far outside"""
+    q, k, v, table, plan, _, dout = _attn_inputs((4, 40, 40, 2, 2, 32, False, 8, 9, True, None), torch.float32)
+    i32 = lambda *x: be.to(torch.tensor(x, dtype=torch.int32))
+    a = [*be.to(q, k, v, table), _plan_on(be, plan)]
+    big = 2 ** 31 - 1
+    for (ql, kl, st), (ql2, kl2, st2) in ((((41, big, -1, 40), (big, 41, 40, -big), (0,) * 4), ((40, 40, 0, 40), (40, 40, 40, 0), (0,) * 4)),
+                                          (((40,) * 4, (40,) * 4, (big, -big, 1 << 30, -(1 << 30))),
+                                           ((40,) * 4, (40,) * 4, (1 << 20, -(1 << 20), 1 << 20, -(1 << 20))))):
+        r = [be.ops.rel_attention(*a, q_lens=i32(*x), k_lens=i32(*y), q_start=i32(*z), return_lse=True)
+             for x, y, z in ((ql, kl, st), (ql2, kl2, st2))]
+        assert torch.equal(r[0][0], r[1][0]) and torch.equal(r[0][1], r[1][1])
+        g = [be.ops.rel_attention_backward(*a, *o, be.to(dout), q_lens=i32(*x), k_lens=i32(*y), q_start=i32(*z))
+             for o, (x, y, z) in zip(r, ((ql, kl, st), (ql2, kl2, st2)))]
+        assert all(torch.equal(x, y) for x, y in zip(*g))
+
+
 def test_rel_attention_taken_out_buckets(be):
     """a table entry at the type's lowest value or -inf takes its bucket out, and a row left with nothing is zeros"""
     for dtype in (torch.float32, torch.bfloat16):
@@ -568,3 +610,91 @@ def test_training_step_through_autograd(be, monkeypatch):
     # sums of L, D and B H L^2 products whose factors carry about (D + L) u each; magnitudes up to the largest gradient
     for g, r in zip(got, want):
         assert float((g.cpu().double() - r).norm() / r.norm()) <= 8 * (D + L) * U
+
+
+# ------------------------------------------------------------------------------------------------------- on the device
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(2, 500, 500, 8, 2, 128, True, 32, 128, False, [(500, 500, 0), (333, 333, 0)]),
+                                  (1, 1100, 1100, 4, 4, 24, False, 32, 300, True, None),
+                                  (4, 1030, 1030, 32, 32, 64, True, 32, 128, False, None),     # more workgroups than walks to cut
+                                  (1, 300, 2000, 6, 2, 96, True, 16, 500, False, [(300, 2000, 1700)])])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rel_attention_larger(hip, case, dtype):
+    _check_attention(hip, case, dtype)
+
+
+@pytest.mark.gpu
+def test_rel_attention_far_offsets(hip):
+    """keys beyond 2^31 elements from the first, across a batch and along one sequence's rows"""
+    D, L = 64, 1 << 15
+    q, table = hip.to(_randn((2, 1, 1, D), 1).bfloat16()), hip.to(_randn((8, 1), 2).bfloat16())
+    plan = RelativeBuckets(8, 40, False, device=hip.device)
+    kv = hip.to(_randn((2, L, 2, D), 3).bfloat16())
+    lens = hip.to(torch.tensor([L, L - 77], dtype=torch.int32))
+    want = hip.ops.rel_attention(q, kv[:, :, :1], kv[:, :, 1:], table, plan, causal=True, k_lens=lens, q_start=lens - 1)
+    for shape, stride in (((2, L, 2, D), (1 << 31, 2 * D, D, 1)), ((2, L, 2, D), (2 * D, 1 << 17, D, 1))):
+        flat = torch.zeros(((shape[0] - 1) * stride[0] + shape[1] * stride[1],), dtype=torch.bfloat16, device=hip.device)
+        far = flat.as_strided(shape, stride)
+        far.copy_(kv)
+        got = hip.ops.rel_attention(q, far[:, :, :1], far[:, :, 1:], table, plan, causal=True, k_lens=lens, q_start=lens - 1)
+        assert torch.equal(got, want)
+        del flat, far
+
+
+@pytest.mark.gpu
+def test_position_operators_in_a_graph_and_on_a_stream(hip):
+    """forward and backward captured twice and replayed in turn between eager calls on other inputs, and everything on a stream
+    of its own (no eager graph of the leaves is alive during a capture: torch does not allow that)"""
+    from occformer_amd import autograd as A
+    B, L, H, D = 2, 200, 4, 64
+    plan = RelativeBuckets(32, 64, True, device=hip.device)
+    cos, sin = rotary_table(256, D)
+    lens = hip.to(torch.tensor([200, 131], dtype=torch.int32))
+    leaves = [hip.to(_randn(s, i)).bfloat16().requires_grad_() for i, s in enumerate([(B, L, 3 * H * D), (D,), (D,), (32, H)])]
+    dout = hip.to(_randn((B, L, H, D), 9)).bfloat16()
+
+    def forward():
+        q, k, v = (t.unflatten(-1, (H, D)) for t in leaves[0].chunk(3, -1))
+        q, k = A.qk_norm_rope(q, k, leaves[1], leaves[2], cos, sin)
+        return A.rel_attention(q, k, v, leaves[3], plan, q_lens=lens, k_lens=lens)
+
+    def step():
+        out = forward()
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        graphs.append((g, outs))
+    for n in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(hip.to(_randn((B, L, 3 * H * D), 50 + n)))
+        want = step()
+        torch.cuda.synchronize()
+        for g, outs in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, outs in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), n
+        with torch.cuda.stream(side):
+            other = step()
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+@pytest.mark.gpu
+def test_position_operators_refuse_mixed_devices(hip):
+    q, w = hip.to(_randn((1, 4, 2, 8), 1)), torch.ones(8)
+    with pytest.raises(OccfError):
+        hip.ops.qk_norm_rope(q, None, w, None)
+    with pytest.raises(OccfError):
+        hip.ops.qk_norm_rope(q.cpu(), None, w, None)
+    plan = RelativeBuckets(8, 9, True, device="cpu")
+    with pytest.raises(OccfError):
+        hip.ops.rel_attention(q, q, q, hip.to(_randn((8, 2), 1)), plan)
