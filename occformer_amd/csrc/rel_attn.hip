@@ -16,20 +16,21 @@
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Many queries: a workgroup owns 128 queries of one head, a wave 32 of them (a lane one query: its running maximum and sum
-// are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.  With two
-// images (NBUF) a tile costs one barrier: the next one is stored while the others still read this one.
+// are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.  Tried beside
+// it at 2 x 4096 causal rows, 16 heads of 64 (104 us) and 8192 of 128 (330 us): a second image and one barrier a tile, 115 and
+// 436 (the offsets cost a wave a SIMD); tiles of 32 keys, 165 and 434; Q K^T of the next tile in one block with this one's
+// exponentials, 144 and 567.
 template <class T, int DP, int KT>
 struct RaFwd {
   static constexpr int tile = 2 * RaType<T>::NT * RaRow<DP>::bytes(KT);                  // K and V
-  static constexpr int NBUF = tile <= 32 * 1024 ? 2 : 1;
-  static size_t bytes(int R) { return NBUF * tile + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
+  static size_t bytes(int R) { return tile + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
 };
 
 template <class T, int DP, int KT>
 __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) rel_attn_fwd_kernel(RaParams p) {
-  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, NBUF = RaFwd<T, DP, KT>::NBUF;
+  constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32;
   OCCF_DYN_SMEM(smem);
-  float* lut = (float*)(smem + NBUF * RaFwd<T, DP, KT>::tile);
+  float* lut = (float*)(smem + RaFwd<T, DP, KT>::tile);
 
   const int tid = threadIdx.x, wave = occf_wave_uniform(tid >> 6), lane = tid & 63, li = lane & 31, lk = lane >> 5;
   const int nqt = (p.Lq + 127) / 128;
@@ -78,30 +79,17 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
     rk.load(kb + k0 * p.ksl, p.ksl, kend - k0, p.D);
     rv.load(vb + k0 * p.vsl, p.vsl, kend - k0, p.D);
   };
-  const auto store = [&](int buf) {
-    rk.store(smem + buf * RaFwd<T, DP, KT>::tile, tid);
-    rv.store(smem + buf * RaFwd<T, DP, KT>::tile + NT * RaRow<DP>::bytes(KT), tid);
-  };
+  const char *img_k = smem, *img_v = smem + NT * RaRow<DP>::bytes(KT);
   const int ntile = (kend + KT - 1) / KT;
   load(0);
   RA_WAIT_LOADS();
-  if (NBUF == 2) {
-    store(0);
-    load(KT);
-  }
   for (int kt = 0; kt < ntile; ++kt) {
     const int k0 = kt * KT;
-    __syncthreads();                                     // this tile is stored, and no wave reads the one before it any more
-    if (NBUF == 1) {
-      store(0);
-      __syncthreads();
-      load(k0 + KT);
-    } else {
-      store((kt + 1) & 1);
-      load(k0 + 2 * KT);
-    }
-    const char* img_k = smem + (NBUF == 2 ? kt & 1 : 0) * RaFwd<T, DP, KT>::tile;
-    const char* img_v = img_k + NT * RaRow<DP>::bytes(KT);
+    __syncthreads();                                     // no wave reads the last tile any more
+    rk.store(smem, tid);
+    rv.store(smem + NT * RaRow<DP>::bytes(KT), tid);
+    __syncthreads();
+    load(k0 + KT);
     if (i0 >= nq || (p.causal && k0 > start + i0 + 31)) continue;      // wave-uniform
     f32x16 s[KT / 32];
     RA_PRIO(1);
