@@ -548,15 +548,19 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// How often the walks are cut: until about two workgroups a compute unit are there (what its registers hold), 128 rows or more
-// a part; twice as many of a causal walk's unequal key tiles (275 instead of 374 us at 2 x 4096, 4 key heads of 64).
-static void ra_bwd_plan(const int64_t* g, int causal, int& qsplit, int& ksplit) {
+// How often the walks are cut, 128 rows or more a part.  A key's: until there are as many workgroups as the card's registers hold
+// (one or two a compute unit, by type and head dim; one beyond that is a second round: 171 instead of 120 us for the whole
+// backward at 2048 rows, 4 heads of 128), twice as many of a causal walk's unequal key tiles (275 instead of 374 us at 2 x 4096, 4
+// key heads of 64).  A query's: one a compute unit, its parts of two matrices cost more than the second one brings (79 instead
+// of 90 us at 3 x 777, 12 heads of 64).
+static void ra_bwd_plan(const int64_t* g, int causal, int dtype, int& qsplit, int& ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
+  const long slots = 256 * (dtype == 0 ? RA_WAVES_PER_SIMD(float, g[5]) : RA_WAVES_PER_SIMD(ra_bf16, g[5]));
   const long wq = B * Hq * ((Lq + 127) / 128), wk = B * Hk * ((Lk + 127) / 128);
   const long mq = (Lk + 127) / 128, mk = (Hq / Hk) * ((Lq + 127) / 128);
   const auto cut = [](long want, long most) { return (int)(want < 1 ? 1 : want > most ? most : want); };
-  qsplit = cut(cut(512 / wq, mq), 8);
-  ksplit = cut(cut((causal ? 1024 : 512) / wk, mk), 16);
+  qsplit = cut(cut(256 / wq, mq), 8);
+  ksplit = cut(cut((causal ? 2 : 1) * slots / wk, mk), 16);
 }
 
 struct RaBwdSizes { long delta, eps, dq, dk, tab; };
@@ -598,7 +602,7 @@ static int ra_bwd(const RaBwd& g, void* stream) {
 extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype) {
   if (ra_check(geom, dtype)) return -1;
   int qs, ks;
-  ra_bwd_plan(geom, causal, qs, ks);
+  ra_bwd_plan(geom, causal, dtype, qs, ks);
   const RaBwdSizes s = ra_bwd_sizes(geom, qs, ks);
   return s.delta + s.eps + s.dq * (dtype == 1 ? 2 : 1) + s.dk * 2 + s.tab;
 }
@@ -624,7 +628,7 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
   p.out = out; p.dout = dout; p.lse = (float*)lse;
   p.dq = dq; p.dk = dk; p.dv = dv;
   g.dtable = dtable;
-  ra_bwd_plan(geom, causal, g.qsplit, g.ksplit);
+  ra_bwd_plan(geom, causal, dtype, g.qsplit, g.ksplit);
   const RaBwdSizes s = ra_bwd_sizes(geom, g.qsplit, g.ksplit);
   p.delta = workspace;
   g.eps = p.delta + s.delta;
