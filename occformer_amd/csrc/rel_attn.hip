@@ -509,13 +509,12 @@ __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
 static void ra_plan(const int64_t* g, int& few, int& nsplit, int& chunk) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
   const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32);
-  static const long tgt = getenv("XTGT") ? atol(getenv("XTGT")) : 512;
   few = rows <= 32 || B * Hq * ((Lq + 127) / 128) < 512;
   nsplit = 1;
   long c = Lk;
   if (few) {
     // about two workgroups a compute unit, none with less than 128 keys (a 32-key tile a wave)
-    long want = (tgt + groups - 1) / groups;
+    long want = (512 + groups - 1) / groups;
     const long most = (Lk + 127) / 128;
     want = want < 1 ? 1 : (want > most ? (most < 1 ? 1 : most) : want);
     want = want > 64 ? 64 : want;
