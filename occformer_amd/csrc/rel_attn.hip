@@ -465,7 +465,8 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
   }
 }
 
-// joins the parts of rel_attn_few_kernel in their order: one thread four columns of a row, a wave of one sequence
+// joins the parts of rel_attn_few_kernel in their order: one thread four columns of a row, a wave of one sequence.
+// All latency (the lengths, then the parts): one pass with a running maximum instead of one for the maxima and one for the sums.
 template <class T>
 __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
   const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
@@ -482,20 +483,36 @@ __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
   const int d = u % (p.D / 4) * 4, rw = u / (p.D / 4), r = rw & 31;
   const long step = (long)p.Hk * nrt * (32 * (p.D + 2));
   const float* ph = p.part + (((long)first * p.Hk + hk) * nrt + (rw >> 5)) * (32 * (p.D + 2));
-  float m = -INFINITY;
-#pragma unroll 8
-  for (int s = 0; s < n; ++s) m = fmaxf(m, ph[s * step + r]);
-  const float mz = m == -INFINITY ? 0.f : m;
-  float l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float a = ra_exp2(ph[s * step + r] - mz);
-    l = fmaf(ph[s * step + 32 + r], a, l);
-    const float4 y = *(const float4*)(ph + s * step + 64 + r * p.D + d);
-    x[0] = fmaf(y.x, a, x[0]);
-    x[1] = fmaf(y.y, a, x[1]);
-    x[2] = fmaf(y.z, a, x[2]);
-    x[3] = fmaf(y.w, a, x[3]);
+  float m = -INFINITY, l = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < n; s0 += 8) {                    // eight parts' loads in flight at once
+    float pm[8], pl[8];
+    float4 y[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const bool ok = s0 + s < n;
+      const float* at = ph + (ok ? s0 + s : n - 1) * step;
+      const float4 z = *(const float4*)(at + 64 + r * p.D + d);
+      pm[s] = ok ? at[r] : -INFINITY;
+      pl[s] = ok ? at[32 + r] : 0.f;
+      y[s] = make_float4(ok ? z.x : 0.f, ok ? z.y : 0.f, ok ? z.z : 0.f, ok ? z.w : 0.f);
+    }
+    float top = m;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) top = fmaxf(top, pm[s]);
+    const float mz = top == -INFINITY ? 0.f : top, old = ra_exp2(m - mz);
+    m = top;
+    l *= old;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] *= old;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float a = ra_exp2(pm[s] - mz);
+      l = fmaf(pl[s], a, l);
+      x[0] = fmaf(y[s].x, a, x[0]);
+      x[1] = fmaf(y[s].y, a, x[1]);
+      x[2] = fmaf(y[s].z, a, x[2]);
+      x[3] = fmaf(y[s].w, a, x[3]);
+    }
   }
   const float inv = l != 0.f ? 1.0f / l : 0.f;
   const int i = rw / G, h = hk * G + rw % G;
