@@ -14,7 +14,7 @@
 // delta: a row of dS sums to zero, but <dO, O> of an O rounded to bf16 (whose P was rounded too) is off by a few 2^-9, and the
 // bias' gradient, sums of dS that nearly cancel, shows it (3.5e-3 of error where its own rounding is 1.7e-3).  The row sums of
 // the dS so formed ARE that error (P sums to one), so the first kernel adds them to the delta that the second one reads, and
-// takes (row sum) x (P K) off its own dQ: one product more, bf16 only; an fp32 O leaves nothing to correct.
+// takes (row sum) x (P K) off its own dQ: one product more, bf16 only; an fp32 O leaves nothing to correct in dQ.
 //
 // Both walks are cut into `splits` where whole ones would not fill the card; rel_attn_finish_kernel adds the parts up in order.
 #include "rel_attn.h"
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
       for (int r = 0; r < 16; ++r) {
         pv[r] = ra_exp2(fmaf(s[r], ce, be));
         ds[r] = pv[r] * dp[r];
-        if (PK) eps += ds[r];
+        eps += ds[r];
       }
       RA_PRIO(1);
 #pragma unroll
@@ -164,11 +164,11 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
       RA_PRIO(0);
     }
   }
-  if (PK) eps += __shfl_xor(eps, 32);
+  eps += __shfl_xor(eps, 32);
   if (i >= p.Lq) return;
   if (lk == 0) {
     if (split == 0) p.delta[stat] = g.qsplit > 1 ? delta : delta + eps;
-    if (PK && g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;      // rel_attn_finish_kernel adds these to delta
+    if (g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;      // rel_attn_finish_kernel adds these to delta
   }
   const long part = (long)split * p.B * p.Lq * p.Hq * p.D + orow;
 #pragma unroll
@@ -482,16 +482,14 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     }
 }
 
-// The parts in order, four columns a thread.  `what` & 1: dq of a walk that was cut (bf16: behind the first kernel, and a row's
-// first thread completes its delta; fp32: with the rest); & 2: behind the second kernel, the bias' gradient on Hq workgroups, then
-// dk and dv where that walk was cut.
+// The parts in order.  Behind the first kernel, where its walk was cut: dq (four columns a thread), and a row's first thread
+// completes its delta.  Behind the second: the bias' gradient on Hq workgroups, then dk and dv where that walk was cut.
 template <class T>
-__global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int what) {
+__global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int dq) {
   const RaParams& p = g.a;
-  constexpr bool PK = RaType<T>::NT == 1;
   const int tid = threadIdx.x;
   int blk = blockIdx.x;
-  if ((what & 2) && blk < p.Hq) {
+  if (!dq && blk < p.Hq) {
     __shared__ float acc[256];
     const int G = p.Hq / p.Hk, hk = blk / G, hg = blk % G;
     int nb2 = 1;
@@ -516,15 +514,13 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
     }
     return;
   }
-  if (what & 2) blk -= p.Hq;
-  const long nq = (long)p.B * p.Lq * p.Hq * p.D, nk = (long)p.B * p.Lk * p.Hk * p.D;
-  const int qblocks = what & 1 ? (int)((nq / 4 + 255) / 256) : 0;
-  const bool dq = blk < qblocks;
-  const long at = ((long)(dq ? blk : blk - qblocks) * 256 + tid) * 4, n = dq ? nq : nk;
+  if (!dq) blk -= p.Hq;
+  const long at = ((long)blk * 256 + tid) * 4;
+  const long n = dq ? (long)p.B * p.Lq * p.Hq * p.D : (long)p.B * p.Lk * p.Hk * p.D;
   if (at >= n) return;
   const int splits = dq ? g.qsplit : g.ksplit;
   const float *pa = dq ? g.dq_part : g.dk_part, *pb = dq ? g.pk_part : g.dv_part;
-  const bool second = !dq || PK;
+  const bool second = !dq || RaType<T>::NT == 1;
   float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < splits; ++s) {
     const float4 a = *(const float4*)(pa + s * n + at);
@@ -535,18 +531,16 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
     }
   }
   if (dq) {
-    if (PK) {
-      const long row = at / p.D;                         // (b Lq + i) Hq + h
-      const int h = (int)(row % p.Hq);
-      const long bi = row / p.Hq;
-      const long stat = (bi / p.Lq * p.Hq + h) * p.Lq + bi % p.Lq;
-      float eps = 0.f;
-      for (int s = 0; s < splits; ++s) eps += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
-      if (at == row * p.D) p.delta[stat] += eps;
+    const long row = at / p.D;                           // (b Lq + i) Hq + h
+    const int h = (int)(row % p.Hq);
+    const long bi = row / p.Hq;
+    const long stat = (bi / p.Lq * p.Hq + h) * p.Lq + bi % p.Lq;
+    float eps = 0.f;
+    for (int s = 0; s < splits; ++s) eps += g.eps[(long)s * p.B * p.Hq * p.Lq + stat];
+    if (at == row * p.D) p.delta[stat] += eps;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = fmaf(-eps, y[e], x[e]);
-    }
-    ra_store4((T*)p.dq + at, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
+    for (int e = 0; e < 4; ++e) x[e] = (second ? fmaf(-eps, y[e], x[e]) : x[e]) * p.scale;
+    ra_store4((T*)p.dq + at, x[0], x[1], x[2], x[3]);
   } else {
     ra_store4((T*)p.dk + at, x[0] * p.scale, x[1] * p.scale, x[2] * p.scale, x[3] * p.scale);
     ra_store4((T*)p.dv + at, y[0], y[1], y[2], y[3]);
@@ -570,12 +564,12 @@ static void ra_bwd_plan(const int64_t* g, int causal, int dtype, int& qsplit, in
 }
 
 struct RaBwdSizes { long delta, eps, dq, dk, tab; };
-static RaBwdSizes ra_bwd_sizes(const int64_t* g, int dtype, int qsplit, int ksplit) {
+static RaBwdSizes ra_bwd_sizes(const int64_t* g, int qsplit, int ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5], nb = g[6];
   RaBwdSizes s;
   const auto up = [](long n) { return (n + 63) / 64 * 64; };             // parts start on 256 bytes
   s.delta = up(B * Hq * Lq);
-  s.eps = qsplit > 1 && dtype == 1 ? up(B * Hq * Lq * qsplit) : 0;
+  s.eps = qsplit > 1 ? up(B * Hq * Lq * qsplit) : 0;
   s.dq = qsplit > 1 ? up(B * Lq * Hq * D * qsplit) : 0;
   s.dk = ksplit > 1 ? up(B * Lk * Hk * D * ksplit) : 0;
   s.tab = up(B * Hq * ksplit * ((Lk + 127) / 128) * nb);
@@ -591,28 +585,25 @@ static int ra_bwd(const RaBwd& g, void* stream) {
                      RaDq<T, DP, KT>::bytes(p.R), stream, g);
   if (rc) return rc;
   const auto blocks = [](long n) { return (unsigned)((n / 4 + 255) / 256); };
-  const auto finish = [&](int what) {
-    const unsigned n = (what & 1 ? blocks((long)p.B * p.Lq * p.Hq * p.D) : 0) +
-                       (what & 2 ? p.Hq + (g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0) : 0);
-    hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(n), dim3(256), 0, (hipStream_t)stream, g, (int)nkt, what);
-    return (int)hipGetLastError();
-  };
-  const bool early = g.qsplit > 1 && RaType<T>::NT == 1;
-  if (early) {
-    rc = finish(1);
+  if (g.qsplit > 1) {
+    hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(blocks((long)p.B * p.Lq * p.Hq * p.D)), dim3(256), 0, (hipStream_t)stream,
+                       g, (int)nkt, 1);
+    rc = (int)hipGetLastError();
     if (rc) return rc;
   }
   rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW>, dim3((unsigned)(p.B * p.Hk * nkt * g.ksplit)), NW * 64,
                  RaDkv<T, DP, QT, NW>::bytes(p.R), stream, g);
   if (rc) return rc;
-  return finish(g.qsplit > 1 && !early ? 3 : 2);
+  hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(p.Hq + (g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0)), dim3(256), 0,
+                     (hipStream_t)stream, g, (int)nkt, 0);
+  OCCF_LAUNCH_CHECK();
 }
 
 extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype) {
   if (ra_check(geom, dtype)) return -1;
   int qs, ks;
   ra_bwd_plan(geom, causal, dtype, qs, ks);
-  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, qs, ks);
+  const RaBwdSizes s = ra_bwd_sizes(geom, qs, ks);
   return s.delta + s.eps + s.dq * (dtype == 1 ? 2 : 1) + s.dk * 2 + s.tab;
 }
 
@@ -638,7 +629,7 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
   p.dq = dq; p.dk = dk; p.dv = dv;
   g.dtable = dtable;
   ra_bwd_plan(geom, causal, dtype, g.qsplit, g.ksplit);
-  const RaBwdSizes s = ra_bwd_sizes(geom, dtype, g.qsplit, g.ksplit);
+  const RaBwdSizes s = ra_bwd_sizes(geom, g.qsplit, g.ksplit);
   p.delta = workspace;
   g.eps = p.delta + s.delta;
   g.dq_part = g.eps + s.eps;
