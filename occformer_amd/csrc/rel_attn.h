@@ -77,6 +77,12 @@ __device__ __forceinline__ f32x16 ra_mm(const RaFrag<NT>& a, const RaFrag<NT>& b
   return occf_mfma_bf16_32x32x16(a.p[0], b.p[0], c);
 }
 
+// bf16 rows times values in two pieces
+__device__ __forceinline__ f32x16 ra_mm(const RaFrag<1>& a, const RaFrag<2>& b, f32x16 c) {
+  c = occf_mfma_bf16_32x32x16(a.p[0], b.p[1], c);
+  return occf_mfma_bf16_32x32x16(a.p[0], b.p[0], c);
+}
+
 __device__ __forceinline__ f32x16 ra_zero16() {
   f32x16 z;
 #pragma unroll
@@ -88,10 +94,12 @@ __device__ __forceinline__ f32x16 ra_zero16() {
 template <int NT>
 __device__ __forceinline__ void ra_split2(float a, float b, uint32_t (&w)[NT]) {
   w[0] = occf_bf16_pack2(a, b);
-  if constexpr (NT == 3) {
+  if constexpr (NT >= 2) {
     a -= occf_u2f(w[0] << 16);
     b -= occf_u2f(w[0] & 0xFFFF0000u);
     w[1] = occf_bf16_pack2(a, b);
+  }
+  if constexpr (NT == 3) {
     a -= occf_u2f(w[1] << 16);
     b -= occf_u2f(w[1] & 0xFFFF0000u);
     w[2] = occf_bf16_pack2(a, b);

@@ -40,7 +40,7 @@ struct RaDq {
   static size_t bytes(int R) { return tile + 4 * (2 * (size_t)R + 1 + 2 * RA_PAD); }
 };
 
-template <class T, int DP, int KT, int NW>
+template <class T, int DP, int KT, int NW, int NP>
 __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq_kernel(RaBwd g) {
   const RaParams& p = g.a;
   constexpr int NT = RaType<T>::NT, KS = DP / 16, DT = DP / 32, TH = NW * 64, QW = NW * 32;
@@ -153,11 +153,12 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
       RA_PRIO(1);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        const RaFrag<NT> df = ra_pack8<NT>(ds + s2 * 8), pf = ra_pack8<NT>(pv + s2 * 8);
+        const RaFrag<NP> df = ra_pack8<NP>(ds + s2 * 8);
+        const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const RaFrag<NT> kt_f = ra_read_trans<NT, DP, KT>(img_k, dt * 32, sub * 2 + s2, lane);
-          acc[dt] = ra_mm<NT>(kt_f, df, acc[dt]);
+          acc[dt] = ra_mm(kt_f, df, acc[dt]);
           if (PK) pk[dt] = ra_mm<NT>(kt_f, pf, pk[dt]);
         }
       }
@@ -206,7 +207,7 @@ struct RaDkv {
   }
 };
 
-template <class T, int DP, int QT, int NW>
+template <class T, int DP, int QT, int NW, int NP>
 __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dkv_kernel(RaBwd g) {
   const RaParams& p = g.a;
   typedef RaDkv<T, DP, QT, NW> L;
@@ -412,11 +413,11 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       }
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8), df = ra_pack8<NT>(ds + s2 * 8);
+        const RaFrag<NP> pf = ra_pack8<NP>(pv + s2 * 8), df = ra_pack8<NP>(ds + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          dv[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_o, dt * 32, sub * 2 + s2, lane), pf, dv[dt]);
-          dk[dt] = ra_mm<NT>(ra_read_trans<NT, DP, QT>(img_q, dt * 32, sub * 2 + s2, lane), df, dk[dt]);
+          dv[dt] = ra_mm(ra_read_trans<NT, DP, QT>(img_o, dt * 32, sub * 2 + s2, lane), pf, dv[dt]);
+          dk[dt] = ra_mm(ra_read_trans<NT, DP, QT>(img_q, dt * 32, sub * 2 + s2, lane), df, dk[dt]);
         }
       }
     }
@@ -576,12 +577,12 @@ static RaBwdSizes ra_bwd_sizes(const int64_t* g, int qsplit, int ksplit) {
   return s;
 }
 
-template <class T, int DP>
-static int ra_bwd(const RaBwd& g, void* stream) {
+template <class T, int DP, int NP>
+static int ra_bwd_run(const RaBwd& g, void* stream) {
   constexpr int NW = 4, KT = RaType<T>::NT == 3 && DP > 64 ? 32 : 64, QT = RaType<T>::NT == 3 ? 32 : 64;
   const RaParams& p = g.a;
   const long nqt = (p.Lq + NW * 32 - 1) / (NW * 32), nkt = (p.Lk + NW * 32 - 1) / (NW * 32);
-  int rc = ra_launch(rel_attn_dq_kernel<T, DP, KT, NW>, dim3((unsigned)(p.B * p.Hq * nqt * g.qsplit)), NW * 64,
+  int rc = ra_launch(rel_attn_dq_kernel<T, DP, KT, NW, NP>, dim3((unsigned)(p.B * p.Hq * nqt * g.qsplit)), NW * 64,
                      RaDq<T, DP, KT>::bytes(p.R), stream, g);
   if (rc) return rc;
   const auto blocks = [](long n) { return (unsigned)((n / 4 + 255) / 256); };
@@ -591,12 +592,22 @@ static int ra_bwd(const RaBwd& g, void* stream) {
     rc = (int)hipGetLastError();
     if (rc) return rc;
   }
-  rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW>, dim3((unsigned)(p.B * p.Hk * nkt * g.ksplit)), NW * 64,
+  rc = ra_launch(rel_attn_dkv_kernel<T, DP, QT, NW, NP>, dim3((unsigned)(p.B * p.Hk * nkt * g.ksplit)), NW * 64,
                  RaDkv<T, DP, QT, NW>::bytes(p.R), stream, g);
   if (rc) return rc;
   hipLaunchKernelGGL(rel_attn_finish_kernel<T>, dim3(p.Hq + (g.ksplit > 1 ? blocks((long)p.B * p.Lk * p.Hk * p.D) : 0)), dim3(256), 0,
                      (hipStream_t)stream, g, (int)nkt, 0);
   OCCF_LAUNCH_CHECK();
+}
+
+// bf16: P and dS go into their products rounded to bf16, or as two bf16 pieces (2^-16) where no walk is longer than 512.  The
+// rounding makes dq, dk and dv about sqrt(2) times as far off as their own rounding alone, and in a short walk, where a few values
+// make up a sum, up to 1.7 times.  Two pieces are one more instruction a product: 45.9 instead of 44.7 us at 2 x 384, 12 heads of
+// 64, but 92.8 instead of 86.1 at 3 x 777 and 546 instead of 459 at 2 x 4096 (forward included, causal, 16 / 4 heads).
+template <class T, int DP>
+static int ra_bwd(const RaBwd& g, void* stream) {
+  if constexpr (RaType<T>::NT == 3) return ra_bwd_run<T, DP, 3>(g, stream);
+  else return g.a.Lq <= 512 && g.a.Lk <= 512 ? ra_bwd_run<T, DP, 2>(g, stream) : ra_bwd_run<T, DP, 1>(g, stream);
 }
 
 extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype) {

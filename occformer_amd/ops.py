@@ -1400,7 +1400,7 @@ class HipOps:
         j <= p_i; other rows, and rows that see no key, are zeros.  A table entry at or below -1e30 takes its bucket out.
         One query of a sequence that grows: q_start = k_lens - 1.  fp32 or bf16 -> [B, Lq, Hq, D]; with ``return_lse`` also the
         rows' base-2 logarithms of the sum of exponentials, fp32 [B, Hq, Lq], for ``rel_attention_backward``.
-        bf16: probabilities are rounded to bf16 before their sum and the product with v."""
+        bf16: probabilities are rounded to bf16 before the product with v, not before their sum."""
         causal = bool(causal)
         (_, dt, geom, scale, need), (q, k, v, _, _, table, lut, q_lens, k_lens, q_start, _) = self._plan(
             self._check_rel_attention, (q, k, v, None, None, table, buckets.lut, q_lens, k_lens, q_start, None),
@@ -1416,7 +1416,8 @@ class HipOps:
     def rel_attention_backward(self, q, k, v, table, buckets, out, lse, dout, scale=None, causal=False, q_lens=None,
                                k_lens=None, q_start=None):
         """-> (dq, dk, dv, dtable) for ``rel_attention``'s out, lse and the gradient dout of out; rows that do not count get
-        zeros.  bf16: P and dS are rounded to bf16 before their products, dtable's sums are not."""
+        zeros.  bf16: P and dS are rounded to bf16 before their products (up to lengths of 512 they go as two bf16 pieces),
+        dtable's sums are not."""
         causal = bool(causal)
         (_, dt, geom, scale, need), (q, k, v, out, dout, table, lut, q_lens, k_lens, q_start, lse) = self._plan(
             self._check_rel_attention, (q, k, v, out, dout, table, buckets.lut, q_lens, k_lens, q_start, lse),

@@ -395,6 +395,31 @@ def test_rel_attention(be, case, dtype):
     _check_attention(be, case, dtype)
 
 
+# walks longer than 512: the bf16 backward rounds P and dS once instead of taking two pieces
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 3, 515, 2, 1, 24, True, 8, 20, False, [(3, 515, 512)]),
+                                  (2, 520, 33, 1, 1, 64, False, 8, 9, True, [(520, 33, 0), (77, 1, -40)]),
+                                  (1, 5, 513, 1, 1, 96, False, 8, 40, True, None),
+                                  (1, 514, 2, 1, 1, 128, True, 8, 9, False, [(513, 2, 0)])])
+def test_rel_attention_long_walks(be, case, dtype):
+    _check_attention(be, case, dtype)
+
+
+@pytest.mark.parametrize("case", [(1, 55, 55, 2, 2, 32, False, 32, 40, True, None), (2, 40, 11, 4, 2, 24, True, 8, 40, False, None),
+                                  (1, 94, 94, 4, 2, 64, True, 16, 40, True, None)])
+def test_rel_attention_short_walks_round_once(be, case):
+    """bf16 gradients of short walks: no further off, in the mean square, than their own last rounding of the exact value and a
+    tenth (what else there is, 2^-16 of dS and P, would have to be 0.45 of it to show)"""
+    q, k, v, table, plan, lens, dout = _attn_inputs(case, torch.bfloat16)
+    ref = _attn_ref(q, k, v, table, plan, case[6], case[5] ** -0.5, *lens, dout, torch.bfloat16)
+    dq, dk, dv, tb, do = be.to(q), be.to(k), be.to(v), be.to(table), be.to(dout)
+    out, lse = be.ops.rel_attention(dq, dk, dv, tb, _plan_on(be, plan), causal=case[6], return_lse=True)
+    got = be.ops.rel_attention_backward(dq, dk, dv, tb, _plan_on(be, plan), out, lse, do, causal=case[6])
+    for name, g in zip(("dq", "dk", "dv", "dtable"), got):
+        want = ref[name][0]
+        assert float((g.cpu().double() - want).norm()) <= 1.1 * float((want.bfloat16().double() - want).norm()), name
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("D,causal", [(24, False), (64, True), (96, False), (128, True)])
 def test_rel_attention_many_rows(be, D, causal, dtype):
