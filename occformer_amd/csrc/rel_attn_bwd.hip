@@ -16,6 +16,10 @@
 // the dS so formed ARE that error (P sums to one), so the first kernel adds them to the delta that the second one reads, and
 // takes (row sum) x (P K) off its own dQ: one product more, bf16 only; an fp32 O leaves nothing to correct in dQ.
 //
+// 2 x 4096 causal bf16 rows, 16 / 4 heads of 64: 152 and 235 us, 900 and 585 TFLOP/s of four products each.  The first kernel is
+// bound by the products and the exponentials beside them, the second by the LDS: its operands come as rows and as columns, and
+// the diagonals' sums go through it.  2 x 1000 fp32 rows, 8 heads of 24: 31 and 46 us, short walks of 256 and 512 workgroups.
+//
 // Both walks are cut into `splits` where whole ones would not fill the card; rel_attn_finish_kernel adds the parts up in order.
 #include "rel_attn.h"
 #include "../../include/occformer_hip.h"
@@ -483,8 +487,9 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     }
 }
 
-// The parts in order.  Behind the first kernel, where its walk was cut: dq (four columns a thread), and a row's first thread
-// completes its delta.  Behind the second: the bias' gradient on Hq workgroups, then dk and dv where that walk was cut.
+// The parts in order, a stream (12.4 us for 75 MB, four parts of 2 x 4096 x 4 heads of 64 keys and values).  Behind the first
+// kernel, where its walk was cut: dq (four columns a thread), and a row's first thread completes its delta.  Behind the second:
+// the bias' gradient on Hq workgroups, then dk and dv where that walk was cut.
 template <class T>
 __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, int dq) {
   const RaParams& p = g.a;
@@ -550,9 +555,9 @@ __global__ void __launch_bounds__(256) rel_attn_finish_kernel(RaBwd g, int nkt, 
 
 // ---------------------------------------------------------------------------------------------------------------------
 // How often the walks are cut, 128 rows or more a part.  A key's: until there are as many workgroups as the card's registers hold
-// (one or two a compute unit, by type and head dim; one beyond that is a second round: 171 instead of 120 us for the whole
-// backward at 2048 rows, 4 heads of 128), twice as many of a causal walk's unequal key tiles (275 instead of 374 us at 2 x 4096, 4
-// key heads of 64).  A query's: one a compute unit, its parts of two matrices cost more than the second one brings (79 instead
+// (one or two a compute unit, by type and head dim; beyond that is a second round: 120 instead of 101 us for the whole
+// backward at 2048 rows, 4 heads of 128), twice as many of a causal walk's unequal key tiles (a quarter off that kernel's time at
+// 2 x 4096, 4 key heads of 64).  A query's: one a compute unit, its parts of two matrices cost more than the second one brings (79 instead
 // of 90 us at 3 x 777, 12 heads of 64).
 static void ra_bwd_plan(const int64_t* g, int causal, int dtype, int& qsplit, int& ksplit) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];

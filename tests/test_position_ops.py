@@ -568,6 +568,20 @@ def test_rel_attention_c_entry_refuses(be):
     assert lib.occf_qk_norm_rope_bwd(*[n] * 14, g, 1e-6, 0, 0, n) < 0
 
 
+def test_qk_norm_rope_c_entry_refuses_axes(be):
+    """two axes whose columns do not fill the table would read a third coordinate that the positions do not have"""
+    import ctypes
+    q, w = be.to(_randn((1, 4, 2, 8), 1), torch.ones(8))
+    cos, sin = be.to(*rotary_table(8, 8, device="cpu"))
+    pos, out = be.to(torch.zeros((4, 2), dtype=torch.int32)), torch.empty_like(q)
+    for axes, cuts in ((2, (2, 3)), (2, (3, 2)), (2, (0, 4)), (3, (0, 2))):
+        g = (ctypes.c_int64 * 17)(1, 4, 2, 0, 8, 8, 8, axes, *cuts, 0, 64, 16, 8, 0, 0, 0)
+        ptr = [t if t is None else t.data_ptr() for t in (q, None, w, None, cos, sin, pos, out, None)]
+        assert be.ops.lib.occf_qk_norm_rope_fwd(*ptr, g, 1e-6, 0, 0, ctypes.c_void_p(0)) < 0
+        ptr = [t if t is None else t.data_ptr() for t in (q, None, w, None, cos, sin, pos, out, None, out, None, w, None, out)]
+        assert be.ops.lib.occf_qk_norm_rope_bwd(*ptr, g, 1e-6, 0, 0, ctypes.c_void_p(0)) < 0
+
+
 def _step(ops, x, w, table, plan, cos, sin, pos, lens, Hq, Hk, D, causal):
     q, k, v = x.split((Hq * D, Hk * D, Hk * D), -1)
     heads = lambda t: t.unflatten(-1, (-1, D))
