@@ -525,26 +525,25 @@ __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// How a call is run.  The few-query kernel wins while the other one's workgroups would not be two a compute unit (4 x 2500
-// fp32 queries of 4 heads, 320 of them: 67 instead of 106 us; 252 at 3 x 777 bf16: 19 instead of 24 us).
-static void ra_plan(const int64_t* g, int& few, int& nsplit, int& chunk) {
-  const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4];
-  const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32);
-  few = rows <= 32 || B * Hq * ((Lq + 127) / 128) < 512;
-  nsplit = 1;
-  long c = Lk;
-  if (few) {
-    // about two workgroups a compute unit, none with less than 128 keys (a 32-key tile a wave)
-    long want = (512 + groups - 1) / groups;
-    const long most = (Lk + 127) / 128;
-    want = want < 1 ? 1 : (want > most ? (most < 1 ? 1 : most) : want);
-    want = want > 64 ? 64 : want;
-    c = (Lk + want - 1) / want;
-    c = (c + 127) / 128 * 128;
-    nsplit = (int)((Lk + c - 1) / c);
-    if (nsplit < 1) nsplit = 1;
-  }
-  chunk = (int)c;
+// How a call is run.  `walks`: workgroups of the kernel for many queries, counted by the keys they can see (causal: about half; own
+// key lengths: as if half).  The few-query kernel takes those calls where there are too few to fill the card, as it cuts the work
+// finer, but it reads the keys once for 32 rows instead of 128 and gains less the wider a head is.  us, few / many queries:
+//   heads of 32:  288 walks, bf16  18 / 20, fp32  40 /  42;  384 walks   37 /  24,  79 /  57
+//   heads of 64:  136 walks, bf16  32 / 41, fp32  74 / 105;  168 walks   23 /  18,  43 /  42
+//   heads of 128:  48 walks, bf16  29 / 41, fp32  86 / 137;  64 walks    21 /  18,  50 /  45
+// Its keys are cut into parts as long as these are no more than two workgroups a compute unit (with a third round at 2 x 400, 16
+// heads of 64 bf16: 23 instead of 12 us), none shorter than what the launch that joins them costs (one query of 8 heads: 333 fp32
+// keys of 24 in one part 11.7, in three 15.3; 700 bf16 keys of 64 10.9 and 16; 512 fp32 keys of 128 in four 16.7, in one 25).
+static void ra_plan(const int64_t* g, int causal, int lengths, int dtype, int& few, int& nsplit, int& chunk) {
+  const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5];
+  const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32), nqt = (Lq + 127) / 128;
+  const long walks = B * Hq * (causal ? nqt + 1 : 2 * nqt) / (lengths && B > 1 ? 4 : 2);
+  few = rows <= 32 || walks < (D <= 32 ? 340 : D <= 64 ? 160 : 56);
+  const long most = Lk / (dtype == 1 ? 512 : D <= 64 ? 256 : 128), want = 512 / groups;
+  nsplit = (int)(want < most ? want : most);
+  nsplit = nsplit < 1 ? 1 : (nsplit > 64 ? 64 : nsplit);
+  chunk = (int)(((Lk + nsplit - 1) / nsplit + 127) / 128 * 128);
+  nsplit = (int)((Lk + chunk - 1) / chunk);
 }
 
 template <class T, int DP>
@@ -570,8 +569,8 @@ static int ra_fwd(RaParams& p, int few, void* stream) {
 extern "C" long occf_rel_attn_workspace(const int64_t* geom, int dtype) {
   if (ra_check(geom, dtype)) return -1;
   int few, nsplit, chunk;
-  ra_plan(geom, few, nsplit, chunk);
-  if (!few || nsplit == 1) return 0;
+  ra_plan(geom, 0, 0, dtype, few, nsplit, chunk);        // (the parts depend on neither the mask nor the lengths)
+  if (nsplit == 1) return 0;
   const long rows = geom[1] * (geom[3] / geom[4]);
   return (long)(nsplit + 1) * geom[0] * geom[4] * ((rows + 31) / 32) * 32 * (geom[5] + 2);
 }
@@ -586,12 +585,12 @@ extern "C" int occf_rel_attn_fwd(const void* q, const void* k, const void* v, co
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) != 0) return OCCF_EINVAL;
   int few;
   RaParams p = ra_params(geom, scale, causal);
-  ra_plan(geom, few, p.nsplit, p.chunk);
+  ra_plan(geom, causal, k_lens != nullptr, dtype, few, p.nsplit, p.chunk);
   const long need = occf_rel_attn_workspace(geom, dtype);
   if (need > 0 && (!workspace || workspace_floats < need)) return OCCF_EINVAL;
   p.q = q; p.k = k; p.v = v; p.table = table; p.lut = lut;
   p.q_lens = q_lens; p.k_lens = k_lens; p.q_start = q_start;
-  p.o = out; p.lse = lse; p.part = need > 0 ? workspace : nullptr;
+  p.o = out; p.lse = lse; p.part = few && need > 0 ? workspace : nullptr;
   p.by_length = p.part && k_lens && p.B > 1 && p.B <= 512;
   p.units = p.B * (p.nsplit + p.by_length);
   RA_DISPATCH(dtype, p.D, ra_fwd, p, few, stream);

@@ -429,6 +429,14 @@ def test_rel_attention_many_rows(be, D, causal, dtype):
     _check_attention(be, (13, 40, 70, 10, 5, D, causal, 8, 12, not causal, rows), dtype, backward=False)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 36, 70, 344, 172, 24, False, 8, 12, True, [(33, 65, 0)]),
+                                  (1, 36, 70, 176, 44, 64, True, 8, 12, False, [(36, 70, 34)])])
+def test_rel_attention_many_heads(be, case, dtype):
+    """enough heads of 32 and 64 columns that the kernel for many queries takes them"""
+    _check_attention(be, case, dtype, backward=False)
+
+
 @pytest.mark.parametrize("Lq", [260, 129])
 def test_rel_attention_causal_tiles(be, Lq):
     """causal, several tiles of 128 queries and more heads than one round of the workgroups' order takes"""
@@ -464,6 +472,18 @@ def test_rel_attention_single_queries(be, case, dtype):
         # the same keys in other parts: as in test_prompt_then_single_tokens
         tol = (3 * BF if dtype == torch.bfloat16 else (4 * Lk + 8 * D) * U) * float(v.abs().amax())
         assert float((want - got).abs().max()) <= tol
+
+
+# keys in several parts, of either type
+LONG_SINGLE = [(2, 1030, 1, 1, 32, None), (3, 1100, 4, 2, 24, [1100, 0, 129]), (5, 1030, 17, 1, 64, [1, 127, 128, 1030, 400]),
+               (70, 1030, 2, 1, 8, [(37 * b) % 1031 for b in range(70)]), (2, 2060, 32, 1, 128, [260, 2060])]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", LONG_SINGLE)
+def test_rel_attention_single_queries_long(be, case, dtype):
+    """by parts of the keys: the wave that joins them, parts by the sequences' lengths, sequences of none"""
+    test_rel_attention_single_queries(be, case, dtype)
 
 
 def test_rel_attention_lengths_out_of_range(be):
