@@ -1203,13 +1203,17 @@ class HipOps:
             raise OccfError(f"{what}: fp32 or bf16 tensors expected, got {first.dtype}")
         return self._DTYPES[first.dtype]
 
-    def _launch_on(self, t, name, *args):
-        """``_call`` with the stream of the tensors' own device, which need not be the current one"""
-        if self.strict and t.device.index != torch.cuda.current_device():
-            with torch.cuda.device(t.device):
-                self._call(name, *args, self._stream())
-        else:
-            self._call(name, *args, self._stream())
+    def _launch_on(self, name, tensors, *args):
+        """``_call`` with the tensors' addresses (the first one is never None) and the stream of their own device, which need not
+        be the current one"""
+        at = [None if t is None else t.data_ptr() for t in tensors]
+        if not self.strict:
+            return self._call(name, *at, *args, None)
+        device = tensors[0].device.index
+        if device == torch.cuda.current_device():
+            return self._call(name, *at, *args, _raw_stream(device))
+        with torch.cuda.device(device):
+            self._call(name, *at, *args, _raw_stream(device))
 
     def _plan(self, check, tensors, *rest):
         """``check(*tensors, *rest)`` -> (plan, tensors as the kernels take them), once per layout: shapes, strides, types and
@@ -1218,7 +1222,7 @@ class HipOps:
         beside a kernel of 3 for a single token)."""
         key = (check.__name__, rest, *[None if t is None else (t.shape, t.stride(), t.dtype, t.device) for t in tensors])
         plan = self._plans.get(key)
-        if plan is not None and self._direct(plan[0], tensors):
+        if plan is not None and (plan[0][0] == 1 or self._direct(plan[0], tensors)):
             return plan, tensors
         plan, taken = check(*tensors, *rest)
         if all(x is y for x, y in zip(tensors, taken)):
@@ -1322,9 +1326,7 @@ class HipOps:
             "qk_norm_rope")
         qo = torch.empty_like(q, memory_format=torch.contiguous_format)
         ko = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-        P = self._address
-        self._launch_on(q, "occf_qk_norm_rope_fwd", P(q), P(k), P(qw), P(kw), P(cos), P(sin), P(positions), P(qo), P(ko),
-                        geom, float(eps), interleaved, dt)
+        self._launch_on("occf_qk_norm_rope_fwd", (q, k, qw, kw, cos, sin, positions, qo, ko), geom, float(eps), interleaved, dt)
         return qo, ko
 
     def qk_norm_rope_backward(self, q, k, q_weight, k_weight, dq_out, dk_out, cos=None, sin=None, positions=None, eps=1e-6,
@@ -1338,14 +1340,9 @@ class HipOps:
         if k is not None:
             dk, dkw = torch.empty_like(dk_out), torch.empty_like(kw)
         ws = self._ws(self.lib.occf_qk_norm_rope_bwd_workspace(q.shape[3]), q.device)
-        P = self._address
-        self._launch_on(q, "occf_qk_norm_rope_bwd", P(q), P(k), P(qw), P(kw), P(cos), P(sin), P(positions), P(dq_out),
-                        P(dk_out), P(dq), P(dk), P(dqw), P(dkw), P(ws), geom, float(eps), interleaved, dt)
+        self._launch_on("occf_qk_norm_rope_bwd", (q, k, qw, kw, cos, sin, positions, dq_out, dk_out, dq, dk, dqw, dkw, ws),
+                        geom, float(eps), interleaved, dt)
         return dq, dk, dqw, dkw
-
-    @staticmethod
-    def _address(t):
-        return None if t is None else t.data_ptr()
 
     @staticmethod
     def _aligned(t):
@@ -1408,9 +1405,8 @@ class HipOps:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=self.f32, device=q.device) if return_lse else None
         ws = torch.empty((need,), dtype=self.f32, device=q.device) if need else None
-        P = self._address
-        self._launch_on(q, "occf_rel_attn_fwd", P(q), P(k), P(v), P(table), P(lut), P(q_lens), P(k_lens), P(q_start), P(out),
-                        P(lse), P(ws), need, geom, scale, causal, dt)
+        self._launch_on("occf_rel_attn_fwd", (q, k, v, table, lut, q_lens, k_lens, q_start, out, lse, ws), need, geom, scale,
+                        causal, dt)
         return (out, lse) if return_lse else out
 
     def rel_attention_backward(self, q, k, v, table, buckets, out, lse, dout, scale=None, causal=False, q_lens=None,
@@ -1427,9 +1423,8 @@ class HipOps:
         dk = torch.empty_like(k, memory_format=torch.contiguous_format)
         dv = torch.empty_like(v, memory_format=torch.contiguous_format)
         ws = torch.empty((need,), dtype=self.f32, device=q.device)
-        P = self._address
-        self._launch_on(q, "occf_rel_attn_bwd", P(q), P(k), P(v), P(table), P(lut), P(q_lens), P(k_lens), P(q_start), P(out),
-                        P(lse), P(dout), P(dq), P(dk), P(dv), P(dtable), P(ws), need, geom, scale, causal, dt)
+        self._launch_on("occf_rel_attn_bwd", (q, k, v, table, lut, q_lens, k_lens, q_start, out, lse, dout, dq, dk, dv, dtable, ws),
+                        need, geom, scale, causal, dt)
         return dq, dk, dv, dtable
 
     # ------------------------------------------------------------------ img_inputs producer (csrc/pipeline.hip)
