@@ -757,3 +757,30 @@ def test_position_operators_refuse_mixed_devices(hip):
     plan = RelativeBuckets(8, 9, True, device="cpu")
     with pytest.raises(OccfError):
         hip.ops.rel_attention(q, q, q, hip.to(_randn((8, 2), 1)), plan)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [2, 16])
+def test_rel_attention_far_rows_training(hip, H):
+    """rows of queries, keys and values beyond 2^31 elements from the first, forward (both kernels) and backward: the same bits as
+    from rows side by side"""
+    L, D, step = 2100, 64, 1 << 20
+    x = hip.to(_randn((1, L, 3, H, D), 41).bfloat16())
+    table, dout = hip.to(_randn((8, H), 42).bfloat16()), hip.to(_randn((1, L, H, D), 43).bfloat16())
+    plan = RelativeBuckets(8, 40, True, device=hip.device)
+    flat = torch.zeros((L * step,), dtype=torch.bfloat16, device=hip.device)
+    far = flat.as_strided((1, L, 3, H, D), (L * step, step, H * D, D, 1))
+    far.copy_(x)
+    got = []
+    for t in (x, far):
+        q, k, v = t.unbind(2)
+        out, lse = hip.ops.rel_attention(q, k, v, table, plan, return_lse=True)
+        got.append((out, lse, *hip.ops.rel_attention_backward(q, k, v, table, plan, out, lse, dout)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    w = torch.ones(D, device=hip.device).bfloat16()
+    cos, sin = rotary_table(L, D, device=hip.device)
+    a, b = ([*hip.ops.qk_norm_rope(t[:, :, 0], t[:, :, 1], w, w, cos, sin),
+             *hip.ops.qk_norm_rope_backward(t[:, :, 0], t[:, :, 1], w, w, dout, dout, cos, sin)] for t in (x, far))
+    for y, z in zip(a, b):
+        assert torch.equal(y, z)
