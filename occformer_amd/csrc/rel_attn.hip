@@ -531,15 +531,17 @@ __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
 //   heads of 32:  288 walks, bf16  18 / 20, fp32  40 /  42;  384 walks   37 /  24,  79 /  57
 //   heads of 64:  136 walks, bf16  32 / 41, fp32  74 / 105;  168 walks   23 /  18,  43 /  42
 //   heads of 128:  48 walks, bf16  29 / 41, fp32  86 / 137;  64 walks    21 /  18,  50 /  45
-// Its keys are cut into parts as long as these are no more than two workgroups a compute unit (with a third round at 2 x 400, 16
-// heads of 64 bf16: 23 instead of 12 us), none shorter than what the launch that joins them costs (one query of 8 heads: 333 fp32
-// keys of 24 in one part 11.7, in three 15.3; 700 bf16 keys of 64 10.9 and 16; 512 fp32 keys of 128 in four 16.7, in one 25).
+// Its keys are cut into parts until three workgroups a compute unit are there (fp32: two, heads beyond 64 columns one, what its
+// registers hold), never a round more: us, so / otherwise:  16 sequences of 8192 bf16 keys, 8 key heads of 128: 106 / 117 with two;
+// 4 of 8192 fp32 keys, 4 key heads of 128: 45 / 56 with two;  2 x 400 bf16, 16 heads of 64: 12 / 23 with a part that fills half
+// a round.  No part is shorter than what the launch that joins them costs: one query of 8 heads, 333 fp32 keys of 24 in one part
+// 11.7, in three 15.3; 700 bf16 keys of 64 10.9 and 16; 512 fp32 keys of 128 in four 16.7, in one 25.
 static void ra_plan(const int64_t* g, int causal, int lengths, int dtype, int& few, int& nsplit, int& chunk) {
   const long B = g[0], Lq = g[1], Lk = g[2], Hq = g[3], Hk = g[4], D = g[5];
   const long rows = Lq * (Hq / Hk), groups = B * Hk * ((rows + 31) / 32), nqt = (Lq + 127) / 128;
   const long walks = B * Hq * (causal ? nqt + 1 : 2 * nqt) / (lengths && B > 1 ? 4 : 2);
   few = rows <= 32 || walks < (D <= 32 ? 340 : D <= 64 ? 160 : 56);
-  const long most = Lk / (dtype == 1 ? 512 : D <= 64 ? 256 : 128), want = 512 / groups;
+  const long most = Lk / (dtype == 1 ? 768 : D <= 64 ? 256 : 128), want = (dtype == 1 ? 768 : D <= 64 ? 512 : 256) / groups;
   nsplit = (int)(want < most ? want : most);
   nsplit = nsplit < 1 ? 1 : (nsplit > 64 ? 64 : nsplit);
   chunk = (int)(((Lk + nsplit - 1) / nsplit + 127) / 128 * 128);

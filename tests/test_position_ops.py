@@ -476,7 +476,8 @@ def test_rel_attention_single_queries(be, case, dtype):
 
 # keys in several parts, of either type
 LONG_SINGLE = [(2, 1030, 1, 1, 32, None), (3, 1100, 4, 2, 24, [1100, 0, 129]), (5, 1030, 17, 1, 64, [1, 127, 128, 1030, 400]),
-               (70, 1030, 2, 1, 8, [(37 * b) % 1031 for b in range(70)]), (2, 2060, 32, 1, 128, [260, 2060])]
+               (70, 1030, 2, 1, 8, [(37 * b) % 1031 for b in range(70)]), (2, 2060, 32, 1, 128, [260, 2060]),
+               (3, 1700, 4, 2, 24, [1700, 0, 129]), (70, 1540, 2, 1, 8, [(37 * b) % 1541 for b in range(70)])]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
