@@ -220,8 +220,9 @@ __device__ __forceinline__ bool ra_unit(const RaParams& p, int unit, int seq, in
 // waits for another before the join at the end.  (Keys through LDS, in whole rows of the cache line, took 99 instead of 67 us for
 // 4 x 2500 fp32 queries and as long for single ones.)  Bound by the stream of keys and values: 16 rows take half the
 // accumulators, products and exponentials of 32, which leaves room for a second tile in flight.  16 sequences of up to 8192 bf16
-// keys, 8 key heads of 128: 53 us, 5.4 TB/s; 4 x 2500 fp32 queries and keys, 4 heads of 32: 61 us, bound by the six products a
-// score and their operands' splitting.
+// keys, 8 key heads of 128: 46 us a launch among others on the same keys, part of them still cached, 67 us a call (with the join)
+// on others; 4 x 2500 fp32 queries and keys, 4 heads of 32: 61 us, bound by the six products a score and their operands'
+// splitting.
 // part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
 template <class T, int DP, int RW>
 struct RaFew {
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
 
 // joins the parts of rel_attn_few_kernel in their order: one thread four columns of a row, a wave of one sequence.
 // All latency (the lengths, then the parts): one pass with a running maximum instead of one for the maxima and one for the sums
-// (7.3 instead of 8.5 us for 512 rows of 128).
+// (7.3 instead of 8.5 us for four parts of 512 rows of 128).
 template <class T>
 __global__ void __launch_bounds__(256) rel_attn_join_kernel(RaParams p) {
   const int G = p.Hq / p.Hk, rows = p.Lq * G, nrt = (rows + 31) / 32;
