@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
     ro.store(to + NT * RaRow<DP>::bytes(QT), tid);
     float *s_lse = (float*)(to + L::images), *s_delta = s_lse + QT;
     if (tid < QT) {
-      // rows that do not count or see no key: P = 0
+      // rows that do not count or see no key: P = 0 (the former are hidden as well: a row of zeros times an infinite key is NaN)
       const bool row = nrow + tid < nend;
       s_lse[tid] = !row || nlse == -INFINITY ? -INFINITY : LSE_FIRST ? -nlse / p.c : -nlse;
       s_delta[tid] = -ndelta;
@@ -384,8 +384,8 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       const int pl = start + i0 + 4 * lk;                // position of row 0 of this lane
       float ce, be;
       ra_bias_mask<-1>(s, lut + (near ? j - pl + p.R + RA_PAD : 32), near, rel0 > 0 ? far_above : far_below,
-                       j0 + 32 > nk || (p.causal && rel0 + 31 > 0), p.c, ce, be,
-                       [&](int o) { return !live || (p.causal && j > pl + o); });
+                       j0 + 32 > nk || i0 + 32 > nq || (p.causal && rel0 + 31 > 0), p.c, ce, be,
+                       [&](int o) { return !live || pl + o >= start + nq || (p.causal && j > pl + o); });
       float ds[16], pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {

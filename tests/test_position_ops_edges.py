@@ -1,0 +1,40 @@
+"""Position operators where a value, a row or a layout is out of the ordinary: infinities and the largest numbers, rows and keys
+that nothing reaches, long sums, refusals.  Definitions and bounds as in test_position_ops.py."""
+import math
+
+import pytest
+import torch
+
+from tests.test_position_ops import BF, NAN, U, _attn_inputs, _attn_ref, _half, _plan_on, _randn, _within
+
+# few queries; enough heads that the kernel for many queries takes the call (B, Lq, Lk, Hq, Hk, D, causal, buckets, radius, both
+# sides, rows)
+FEW = (1, 40, 40, 2, 2, 32, False, 8, 9, True, [(40, 39, 0)])
+MANY = (1, 40, 40, 56, 28, 128, False, 8, 9, True, [(40, 39, 0)])
+
+
+def _last_key_hidden(be, case, dtype, low):
+    """a call whose last key is hidden by ``low`` in a column where every query is 1, and the reference without that key"""
+    q, k, v, table, plan, lens, dout = _attn_inputs(case, dtype)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[:, -1], v[:, -1] = 0.5, 2.0
+    k[:, -1, :, 0] = low
+    want = k.clone()
+    want[:, -1] = 0.0
+    return q, k, v, table, plan, dout, _attn_ref(q, want, v, table, plan, case[6], case[5] ** -0.5, *lens, dout, dtype)
+
+
+
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+def test_rel_attention_rows_behind_the_last_meet_an_infinite_key(be, low):
+    """a mask as one more column of the keys, bf16: the rows that fill the last tile of 40 queries are zeros, and zero times -inf is
+    no number (nor is it a term of these gradients; dq's column of the mask has none, by definition)"""
+    low = torch.finfo(torch.bfloat16).min if low == "lowest" else -math.inf
+    q, k, v, table, plan, dout, ref = _last_key_hidden(be, FEW, torch.bfloat16, low)
+    a = [*be.to(q, k, v, table), _plan_on(be, plan)]
+    out, lse = be.ops.rel_attention(*a, return_lse=True)
+    _within(out, *ref["out"], "out")
+    grads = dict(zip(("dq", "dk", "dv", "dtable"), be.ops.rel_attention_backward(*a, out, lse, be.to(dout))))
+    for name, g in grads.items():
+        cut = slice(1, None) if name == "dq" and low == -math.inf else slice(None)
+        _within(g[..., cut], ref[name][0][..., cut], ref[name][1][..., cut], name)
