@@ -10,6 +10,12 @@
 // Products: bf16 inputs are one product.  fp32 inputs are split into three bf16 pieces (x = h + m + l, 24 bits) and a
 // product is the six terms above 2^-24; the two-piece, three-term form the other attention kernels use leaves 3e-6 ... 5e-6
 // of error, which the position bias' gradient (sums with cancellation) would show.
+//
+// An infinity has no second and third piece (inf - inf), and as a first piece it meets the other operand's second, which may be zero
+// or of the other sign.  What is loaded from q, k, v and dO is therefore split with its first two pieces kept finite: what is left
+// over, infinite or NaN, is the third piece, which meets the other operand's first piece alone.  So are values that round to a bf16
+// infinity (beyond 3.39e38, the lowest fp32 number as a mask among them).  Two v_med3 a value; finite values up to there keep
+// their bits.  Left: a product that passes the largest float 2^9 times over may be NaN instead of an infinity.
 #pragma once
 #include "occf_common.h"
 
@@ -106,6 +112,25 @@ __device__ __forceinline__ void ra_split2(float a, float b, uint32_t (&w)[NT]) {
   }
 }
 
+// the same of values from memory, which may be infinite: the first two pieces finite
+__device__ __forceinline__ float ra_clamp(float x, float most) {
+#ifdef OCCF_EMU
+  return x != x ? -most : fminf(fmaxf(x, -most), most);
+#else
+  return __builtin_amdgcn_fmed3f(x, -most, most);
+#endif
+}
+__device__ __forceinline__ void ra_split2_any(float a, float b, uint32_t (&w)[3]) {
+  const float h = 0x1.FEp127f, m = 0x1p120f;             // the largest bf16; the most that rounding a finite value to it leaves
+  w[0] = occf_bf16_pack2(ra_clamp(a, h), ra_clamp(b, h));
+  a -= occf_u2f(w[0] << 16);
+  b -= occf_u2f(w[0] & 0xFFFF0000u);
+  w[1] = occf_bf16_pack2(ra_clamp(a, m), ra_clamp(b, m));
+  a -= occf_u2f(w[1] << 16);
+  b -= occf_u2f(w[1] & 0xFFFF0000u);
+  w[2] = occf_bf16_pack2(a, b);
+}
+
 struct RaU4 { uint32_t x[4]; };
 __device__ __forceinline__ bf16x8 ra_as_frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const RaU4 u = {{a, b, c, d}};
@@ -118,12 +143,15 @@ __device__ __forceinline__ bf16x8 ra_as_frag(uint32_t a, uint32_t b, uint32_t c,
 #endif
 }
 
-// eight consecutive register values -> B operand
-template <int NT>
+// eight consecutive register values -> B operand (ANY: eight from memory, fp32)
+template <int NT, bool ANY = false>
 __device__ __forceinline__ RaFrag<NT> ra_pack8(const float* v) {
   uint32_t w[4][NT];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) ra_split2<NT>(v[2 * e], v[2 * e + 1], w[e]);
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (ANY) ra_split2_any(v[2 * e], v[2 * e + 1], w[e]);
+    else ra_split2<NT>(v[2 * e], v[2 * e + 1], w[e]);
+  }
   RaFrag<NT> f;
 #pragma unroll
   for (int t = 0; t < NT; ++t) f.p[t] = ra_as_frag(w[0][t], w[1][t], w[2][t], w[3][t]);
@@ -148,7 +176,7 @@ __device__ __forceinline__ RaFrag<RaType<T>::NT> ra_row_frag(const T* p, bool ok
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
       f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     }
-    return ra_pack8<3>(f);
+    return ra_pack8<3, true>(f);
   }
 }
 
@@ -233,8 +261,8 @@ struct RaTileRegs {
         *(bf16x8*)to = ra_as_frag(x[n].x[0], x[n].x[1], x[n].x[2], x[n].x[3]);
       } else {
         uint32_t a[3], b[3];
-        ra_split2<3>(occf_u2f(x[n].x[0]), occf_u2f(x[n].x[1]), a);
-        ra_split2<3>(occf_u2f(x[n].x[2]), occf_u2f(x[n].x[3]), b);
+        ra_split2_any(occf_u2f(x[n].x[0]), occf_u2f(x[n].x[1]), a);
+        ra_split2_any(occf_u2f(x[n].x[2]), occf_u2f(x[n].x[3]), b);
 #pragma unroll
         for (int t = 0; t < 3; ++t) {
           const ra_u2 w = {a[t], b[t]};
@@ -265,7 +293,7 @@ __device__ __forceinline__ RaFrag<3> ra_raw_frag(const RaRaw<float>& w) {
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = occf_u2f(w.x[e >> 2].x[e & 3]);
-  return ra_pack8<3>(f);
+  return ra_pack8<3, true>(f);
 }
 
 // ds_read_b64_tr_b16: lane 4 r + q of a 16-lane group gives the address of row r, columns 4 q .. 4 q + 3 of a 4 x 16 block;

@@ -38,3 +38,54 @@ def test_rel_attention_rows_behind_the_last_meet_an_infinite_key(be, low):
     for name, g in grads.items():
         cut = slice(1, None) if name == "dq" and low == -math.inf else slice(None)
         _within(g[..., cut], ref[name][0][..., cut], ref[name][1][..., cut], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("low", ["lowest", "-inf"])
+@pytest.mark.parametrize("case", [FEW, MANY])
+def test_rel_attention_key_hidden_by_a_column(be, case, low, dtype):
+    """a mask as one more column of the keys: the lowest number of the type, or -inf (whose product with the zeros of dS leaves
+    that column of dq without a value, by definition)"""
+    low = torch.finfo(dtype).min if low == "lowest" else -math.inf
+    q, k, v, table, plan, dout, ref = _last_key_hidden(be, case, dtype, low)
+    a = [*be.to(q, k, v, table), _plan_on(be, plan)]
+    out, lse = be.ops.rel_attention(*a, return_lse=True)
+    _within(out, *ref["out"], "out")
+    _within(lse, *ref["lse"], "lse")
+    if case is MANY:
+        return
+    grads = dict(zip(("dq", "dk", "dv", "dtable"), be.ops.rel_attention_backward(*a, out, lse, be.to(dout))))
+    for name, g in grads.items():
+        cut = slice(1, None) if name == "dq" and low == -math.inf else slice(None)
+        _within(g[..., cut], ref[name][0][..., cut], ref[name][1][..., cut], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [FEW, MANY])
+def test_rel_attention_infinite_values(be, case, dtype):
+    """an infinity in one column of v, two that meet in another, a NaN in a third: these columns, and nothing else, show it"""
+    q, k, v, table, plan, lens, _ = _attn_inputs(case, dtype)
+    ref = _attn_ref(q, k, v, table, plan, case[6], case[5] ** -0.5, *lens, None, dtype)
+    v[:, 7, :, 3], v[:, 8, :, 4], v[:, 20, :, 4], v[:, 30, :, 5], v[:, 9, :, 6] = math.inf, math.inf, -math.inf, NAN, -math.inf
+    out = be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), k_lens=be.to(lens[1])).cpu()
+    assert bool((out[..., 3] == math.inf).all()) and bool((out[..., 6] == -math.inf).all())
+    assert bool(out[..., 4].isnan().all()) and bool(out[..., 5].isnan().all())
+    other = [c for c in range(case[5]) if c not in (3, 4, 5, 6)]
+    _within(out[..., other], ref["out"][0][..., other], ref["out"][1][..., other], "out")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [FEW, MANY])
+def test_rel_attention_nan_reaches_its_rows(be, case, dtype):
+    """a NaN in a query shows in its row alone, one in a key in every row that sees it"""
+    q, k, v, table, plan, lens, _ = _attn_inputs(case, dtype)
+    ref = _attn_ref(q, k, v, table, plan, case[6], case[5] ** -0.5, *lens, None, dtype)
+    kw = dict(k_lens=be.to(lens[1]))
+    q[:, 5, 0, 1] = NAN
+    out = be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), **kw).cpu()
+    assert bool(out[:, 5, 0].isnan().all())
+    rest = torch.ones(out.shape[:3], dtype=torch.bool)
+    rest[:, 5, 0] = False
+    _within(out[rest], ref["out"][0][rest], ref["out"][1][rest], "out")
+    k[:, 11, :, 2] = NAN
+    assert bool(be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), **kw).isnan().all())
