@@ -407,8 +407,8 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
   }
 #pragma unroll
   for (int mm = RW; mm < 64; mm <<= 1) l += __shfl_xor(l, mm);
-  if (!live) {                                           // rows behind the last query went along with their tile
-    l = 0.f;
+  if (!live || l == 0.f) {                               // rows behind the last query, or without a key here, went along with
+    l = 0.f;                                             // their tile: 0 times an infinite value is no zero
     m = -INFINITY;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)

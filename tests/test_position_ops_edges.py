@@ -89,3 +89,24 @@ def test_rel_attention_nan_reaches_its_rows(be, case, dtype):
     _within(out[rest], ref["out"][0][rest], ref["out"][1][rest], "out")
     k[:, 11, :, 2] = NAN
     assert bool(be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), **kw).isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 35, 40, 1, 1, 96, True, 8, 20, False, [(35, 40, -5)]),
+                                  (1, 3, 1030, 1, 1, 32, True, 8, 20, False, [(3, 1030, -1)]),      # keys in parts
+                                  (1, 40, 40, 56, 28, 128, True, 8, 9, False, [(40, 40, -5)])])     # the kernel for many queries
+def test_rel_attention_rows_without_keys_beside_an_infinity(be, case, dtype):
+    """rows that stand before every key are zeros whatever the keys of their tile hold; so is a head whose buckets are all out"""
+    q, k, v, table, plan, lens, _ = _attn_inputs(case, dtype)
+    ref = _attn_ref(q, k, v, table, plan, True, case[5] ** -0.5, *lens, None, dtype)
+    v[:, 0, :, 3] = math.inf
+    a = be.to(q, k, v)
+    kw = dict(causal=True, return_lse=True, q_start=be.to(lens[2]))
+    out, lse = be.ops.rel_attention(*a, be.to(table), _plan_on(be, plan), **kw)
+    first = -int(lens[2][0])
+    assert bool((out[:, :first] == 0).all()) and bool((lse[..., :first] == -math.inf).all())
+    assert bool((out[:, first:, :, 3] == math.inf).all())
+    cols = [c for c in range(case[5]) if c != 3]
+    _within(out[..., cols], ref["out"][0][..., cols], ref["out"][1][..., cols], "out")
+    out, lse = be.ops.rel_attention(*a, be.to(torch.full_like(table, -math.inf)), _plan_on(be, plan), **kw)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
