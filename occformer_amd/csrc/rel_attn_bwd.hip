@@ -90,6 +90,7 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   const long stat = ((long)b * p.Hq + h) * p.Lq + ic;
   float lse = live ? p.lse[stat] : INFINITY;
   if (lse == -INFINITY) lse = INFINITY;                  // no key: P = 0
+  const bool some = lse != INFINITY;
   const f32x16 dp_first = ra_splat16(-delta);
 
   int kend = nk;
@@ -171,6 +172,13 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dq
   }
   eps += __shfl_xor(eps, 32);
   if (i >= p.Lq) return;
+  if (!some) {                                           // went along with their tile: 0 times an infinite key is no zero
+    delta = eps = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = ra_zero16();
+#pragma unroll
+    for (int dt = 0; dt < (PK ? DT : 1); ++dt) pk[dt] = ra_zero16();
+  }
   if (lk == 0) {
     if (split == 0) p.delta[stat] = g.qsplit > 1 ? delta : delta + eps;
     if (g.qsplit > 1) g.eps[(long)split * p.B * p.Hq * p.Lq + stat] = eps;      // rel_attn_finish_kernel adds these to delta

@@ -110,3 +110,22 @@ def test_rel_attention_rows_without_keys_beside_an_infinity(be, case, dtype):
     _within(out[..., cols], ref["out"][0][..., cols], ref["out"][1][..., cols], "out")
     out, lse = be.ops.rel_attention(*a, be.to(torch.full_like(table, -math.inf)), _plan_on(be, plan), **kw)
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 40, 40, 1, 1, 32, True, 8, 9, False, [(37, 40, -5)]),
+                                  (1, 9, 300, 1, 1, 24, True, 8, 9, False, [(7, 300, -3)]),          # keys in parts
+                                  (2, 40, 20, 2, 1, 64, False, 8, 9, True, [(33, 20, 0), (0, 20, 0)])])
+def test_rel_attention_backward_rows_that_do_not_count_beside_an_infinity(be, case, dtype):
+    """dq of rows behind the last query, and of rows that see no key, is zero whatever the keys and values hold"""
+    q, k, v, table, plan, lens, dout = _attn_inputs(case, dtype)
+    k[:, 0, :, 2], v[:, 0, :, 3], v[:, 1, :, 4] = math.inf, -math.inf, NAN
+    a = [*be.to(q, k, v, table), _plan_on(be, plan)]
+    kw = dict(causal=case[6], **dict(zip(("q_lens", "k_lens", "q_start"), be.to(*lens))))
+    out, lse = be.ops.rel_attention(*a, return_lse=True, **kw)
+    dq, dk, dv, dtable = be.ops.rel_attention_backward(*a, out, lse, be.to(dout), **kw)
+    for b, (n, m, start) in enumerate(case[10]):
+        unseen = max(0, -start) if case[6] else 0
+        assert bool((out[b, n:] == 0).all()) and bool((out[b, :unseen] == 0).all())
+        assert bool((dq[b, n:] == 0).all()) and bool((dq[b, :unseen] == 0).all())
+        assert n == 0 or bool(dq[b, unseen:n].isnan().any())
