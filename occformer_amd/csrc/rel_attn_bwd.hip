@@ -244,6 +244,10 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
   const int hk = bh % p.Hk, b = bh / p.Hk;
   int nq, nk, start;
   ra_lengths(p, b, nq, nk, start);
+  if (p.causal) {                                        // keys behind the last query: nobody sees them, nor are they looked at
+    const int last = start + nq;
+    nk = last < nk ? (last > 0 ? last : 0) : nk;
+  }
 
   const int j0 = kt * KW + wave * 32, j = j0 + li;
   const bool live = j < nk;

@@ -129,3 +129,18 @@ def test_rel_attention_backward_rows_that_do_not_count_beside_an_infinity(be, ca
         assert bool((out[b, n:] == 0).all()) and bool((out[b, :unseen] == 0).all())
         assert bool((dq[b, n:] == 0).all()) and bool((dq[b, :unseen] == 0).all())
         assert n == 0 or bool(dq[b, unseen:n].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 40, 50, 2, 1, 32, True, 8, 9, False, [(40, 40, 0)]),
+                                  (2, 20, 300, 2, 2, 24, True, 8, 9, False, [(20, 40, 20), (11, 6, -5)])])
+def test_rel_attention_backward_keys_behind_the_last_query(be, case, dtype):
+    """causal: what the rows behind the last query's position hold (a cache not filled yet) is not looked at"""
+    q, k, v, table, plan, lens, dout = _attn_inputs(case, dtype)         # (NaN there)
+    ref = _attn_ref(q, k, v, table, plan, True, case[5] ** -0.5, *lens, dout, dtype)
+    a = [*be.to(q, k, v, table), _plan_on(be, plan)]
+    kw = dict(causal=True, q_lens=be.to(lens[0]), q_start=be.to(lens[2]))
+    out, lse = be.ops.rel_attention(*a, return_lse=True, **kw)
+    _within(out, *ref["out"], "out")
+    for name, g in zip(("dq", "dk", "dv", "dtable"), be.ops.rel_attention_backward(*a, out, lse, be.to(dout), **kw)):
+        _within(g, *ref[name], name)
