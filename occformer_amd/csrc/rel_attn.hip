@@ -128,15 +128,14 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[dt][r] *= a;
     }
+    float sum = 0.f;
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       float pv[16];
       const float off = be[sub] - mref;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        pv[r] = ra_exp2(fmaf(s[sub][r], ce[sub], off));
-        l += pv[r];
-      }
+      for (int r = 0; r < 16; ++r) pv[r] = ra_exp2(fmaf(s[sub][r], ce[sub], off));
+      sum += ra_sum<16>(pv);
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
@@ -145,6 +144,7 @@ __global__ void __launch_bounds__(256, RaType<T>::NT == 1 || DP <= 64 ? 2 : 1) r
           acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, KT>(img_v, dt * 32, sub * 2 + s2, lane), pf, acc[dt]);
       }
     }
+    l += sum;
   }
   l += __shfl_xor(l, 32);
   if (i >= p.Lq) return;
@@ -391,10 +391,8 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
     }
     float pv[NE];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      pv[e] = ra_exp2(s[e] - mref);
-      l += pv[e];
-    }
+    for (int e = 0; e < NE; ++e) pv[e] = ra_exp2(s[e] - mref);
+    l += ra_sum<NE>(pv);
 #pragma unroll
     for (int s2 = 0; s2 < NE / 8; ++s2) {
       const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);

@@ -144,3 +144,24 @@ def test_rel_attention_backward_keys_behind_the_last_query(be, case, dtype):
     _within(out, *ref["out"], "out")
     for name, g in zip(("dq", "dk", "dv", "dtable"), be.ops.rel_attention_backward(*a, out, lse, be.to(dout), **kw)):
         _within(g, *ref[name], name)
+
+
+@pytest.mark.gpu
+def test_rel_attention_sum_of_many_probabilities(hip):
+    """the softmax sum over 32768 keys in one walk.  The values are 1 at 64 keys and 0 elsewhere, so that an output is a short sum
+    over the long one.  T = 512 tiles are added onto a lane's running sum: rounding errors of u at its size then, independent, grow to
+    u sqrt(T) / 3 = 7.5 u, over the two lanes of a row 5.3 u; a probability, the short sum, logarithms and the quotient add 3 u.
+    (One probability after another: 16384 additions, 30 u.)  Bound: twice the former, 17 u."""
+    L, H, D = 32768, 512, 24
+    q, k = hip.to(_randn((1, 33, H, D), 51, 1.5)), hip.to(_randn((1, L, 8, D), 52))
+    v = torch.zeros((1, L, 8, D), device=hip.device)
+    v[:, -64:] = 1.0
+    plan = _plan_on(hip, _attn_inputs(FEW, torch.float32)[4])
+    table = torch.zeros((8, H), device=hip.device)
+    out = hip.ops.rel_attention(q, k, v, table, plan)
+    worst = []
+    for h in range(0, H, 37):
+        p = torch.softmax(q[0, :, h].double() @ k[0, :, h // 64].double().t() * D ** -0.5, -1)
+        want = p[:, -64:].sum(-1, keepdim=True)
+        worst.append(((out[0, :, h].double() - want) / want).square().mean())
+    assert float(torch.stack(worst).mean().sqrt()) <= 17 * U
