@@ -394,10 +394,13 @@ __global__ void __launch_bounds__(NW * 64, RA_WAVES_PER_SIMD(T, DP)) rel_attn_dk
       RA_PRIO(0);
       const bool near = rel0 - 31 < p.R && rel0 + 31 > -p.R;
       const int pl = start + i0 + 4 * lk;                // position of row 0 of this lane
+      // rows [lo, lo + n) of it count: the queries before the last, causal: at or behind the key
+      const int lo = p.causal && j > pl ? j - pl : 0, end = live ? start + nq - pl : 0;
+      const unsigned n = end > lo ? end - lo : 0;
       float ce, be;
       ra_bias_mask<-1>(s, lut + (near ? j - pl + p.R + RA_PAD : 32), near, rel0 > 0 ? far_above : far_below,
                        j0 + 32 > nk || i0 + 32 > nq || (p.causal && rel0 + 31 > 0), p.c, ce, be,
-                       [&](int o) { return !live || pl + o >= start + nq || (p.causal && j > pl + o); });
+                       [&](int o) { return (unsigned)(o - lo) >= n; });
       float ds[16], pv[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
