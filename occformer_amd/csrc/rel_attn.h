@@ -14,8 +14,8 @@
 // An infinity has no second and third piece (inf - inf), and as a first piece it meets the other operand's second, which may be zero
 // or of the other sign.  What is loaded from q, k, v and dO is therefore split with its first two pieces kept finite: what is left
 // over, infinite or NaN, is the third piece, which meets the other operand's first piece alone.  So are values that round to a bf16
-// infinity (beyond 3.39e38, the lowest fp32 number as a mask among them).  Two v_med3 a value; finite values up to there keep
-// their bits.  Left: a product that passes the largest float 2^9 times over may be NaN instead of an infinity.
+// infinity (beyond 3.39e38, the lowest fp32 number as a mask among them).  Finite values up to there keep their bits.  Left: a
+// product that passes the largest float 2^9 times over may be NaN instead of an infinity.
 #pragma once
 #include "occf_common.h"
 
@@ -130,6 +130,23 @@ __device__ __forceinline__ void ra_split2_any(float a, float b, uint32_t (&w)[3]
   b -= occf_u2f(w[1] & 0xFFFF0000u);
   w[2] = occf_bf16_pack2(a, b);
 }
+template <bool ANY>
+__device__ __forceinline__ void ra_split2_of(float a, float b, uint32_t (&w)[3]) {
+  if constexpr (ANY) ra_split2_any(a, b, w);
+  else ra_split2<3>(a, b, w);
+}
+// does a value of a wave need that: tiles on their way into LDS are looked at in half an instruction a value (v_max3 of the
+// magnitudes), and split without the clamps, which cost two each, where none does (forward and backward of 2 x 1000 fp32 rows,
+// 8 heads of 24: 99.7 us without infinities' meaning, 101.4 so, 104.5 with the clamps throughout)
+__device__ __forceinline__ float ra_max3(float m, uint32_t a, uint32_t b) {
+#ifdef OCCF_EMU
+  return fmaxf(m, fmaxf(fabsf(occf_u2f(a)), fabsf(occf_u2f(b))));
+#else
+  asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(m) : "v"(a), "v"(b));
+  return m;
+#endif
+}
+__device__ __forceinline__ bool ra_large(float m) { return __ballot(m > 0x1.FEp127f) != 0; }
 
 struct RaU4 { uint32_t x[4]; };
 __device__ __forceinline__ bf16x8 ra_as_frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -149,7 +166,7 @@ __device__ __forceinline__ RaFrag<NT> ra_pack8(const float* v) {
   uint32_t w[4][NT];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if constexpr (ANY) ra_split2_any(v[2 * e], v[2 * e + 1], w[e]);
+    if constexpr (NT == 3) ra_split2_of<ANY>(v[2 * e], v[2 * e + 1], w[e]);
     else ra_split2<NT>(v[2 * e], v[2 * e + 1], w[e]);
   }
   RaFrag<NT> f;
@@ -252,6 +269,17 @@ struct RaTileRegs {
       x[n] = ra_buf16(buf, EVEN ? at[0] + n * (TH / PER) * ((uint32_t)stride * (uint32_t)sizeof(T)) : at[EVEN ? 0 : n]);
   }
   __device__ __forceinline__ void store(char* img, int tid) const {
+    if (NT == 3 && ra_large(largest())) put<true>(img, tid);
+    else put<false>(img, tid);
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = 0.f;
+#pragma unroll
+    for (int n = 0; n < NU; ++n) m = ra_max3(ra_max3(m, x[n].x[0], x[n].x[1]), x[n].x[2], x[n].x[3]);
+    return m;
+  }
+  template <bool ANY>
+  __device__ __forceinline__ void put(char* img, int tid) const {
 #pragma unroll
     for (int n = 0; n < NU; ++n) {
       const int u = tid + n * TH, row = u / PER, c = (u % PER) * C;
@@ -261,8 +289,8 @@ struct RaTileRegs {
         *(bf16x8*)to = ra_as_frag(x[n].x[0], x[n].x[1], x[n].x[2], x[n].x[3]);
       } else {
         uint32_t a[3], b[3];
-        ra_split2_any(occf_u2f(x[n].x[0]), occf_u2f(x[n].x[1]), a);
-        ra_split2_any(occf_u2f(x[n].x[2]), occf_u2f(x[n].x[3]), b);
+        ra_split2_of<ANY>(occf_u2f(x[n].x[0]), occf_u2f(x[n].x[1]), a);
+        ra_split2_of<ANY>(occf_u2f(x[n].x[2]), occf_u2f(x[n].x[3]), b);
 #pragma unroll
         for (int t = 0; t < 3; ++t) {
           const ra_u2 w = {a[t], b[t]};
@@ -284,18 +312,19 @@ __device__ __forceinline__ void ra_load_raw(RaRaw<T>& f, occf_bbuf buf, uint32_t
 #pragma unroll
   for (int e = 0; e < (int)sizeof(T) / 2; ++e) f.x[e] = ra_buf16(buf, at + 16u * e);
 }
+template <bool ANY>
 __device__ __forceinline__ RaFrag<1> ra_raw_frag(const RaRaw<ra_bf16>& w) {
   RaFrag<1> f;
   f.p[0] = ra_as_frag(w.x[0].x[0], w.x[0].x[1], w.x[0].x[2], w.x[0].x[3]);
   return f;
 }
+template <bool ANY>
 __device__ __forceinline__ RaFrag<3> ra_raw_frag(const RaRaw<float>& w) {
   float f[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) f[e] = occf_u2f(w.x[e >> 2].x[e & 3]);
-  return ra_pack8<3, true>(f);
+  return ra_pack8<3, ANY>(f);
 }
-
 // ds_read_b64_tr_b16: lane 4 r + q of a 16-lane group gives the address of row r, columns 4 q .. 4 q + 3 of a 4 x 16 block;
 // lane t gets column t, rows 0..3
 #ifdef OCCF_EMU
@@ -409,14 +438,6 @@ __device__ __forceinline__ void ra_bias_mask(f32x16& s, const float* bl, bool ne
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = hide((r & 3) + 8 * (r >> 2)) ? -INFINITY : s[r];
   }
-}
-
-// sum of a lane's N probabilities of a tile, in pairs: added one by one onto a row's running sum they would each round at its size
-// (relative error of that sum over 32768 keys, restated in numpy: 1.2e-6 one by one, 2e-7 by tiles)
-template <int N>
-__device__ __forceinline__ float ra_sum(const float* v) {
-  if constexpr (N == 2) return v[0] + v[1];
-  else return ra_sum<N / 2>(v) + ra_sum<N / 2>(v + N / 2);
 }
 
 __device__ __forceinline__ f32x16 ra_splat16(float x) {
