@@ -10,6 +10,7 @@ the library.  Parameters enter as Function inputs so autograd accumulates into t
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import fused, noise
 from .ops import get_ops
@@ -605,6 +606,7 @@ class QkNormRope(torch.autograd.Function):
         return get_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, axis_dims, interleaved)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         dq_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if dq_out is None else dq_out
@@ -631,6 +633,7 @@ class RelAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, out, lse, q_lens, k_lens, q_start = ctx.saved_tensors
         buckets, scale, causal = ctx.cfg

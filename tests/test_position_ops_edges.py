@@ -165,3 +165,21 @@ def test_rel_attention_sum_of_many_probabilities(hip):
         want = p[:, -64:].sum(-1, keepdim=True)
         worst.append(((out[0, :, h].double() - want) / want).square().mean())
     assert float(torch.stack(worst).mean().sqrt()) <= 17 * U
+
+
+def test_second_derivatives_are_refused(be, monkeypatch):
+    """the gradients come out of kernels that autograd cannot differentiate: asking for it raises, it does not drop the terms"""
+    from occformer_amd import autograd as A
+    monkeypatch.setattr(A, "get_ops", lambda: be.ops)
+    q, k, v, table, plan, _, _ = _attn_inputs(FEW, torch.float32)
+    q, k, v, table = (t.nan_to_num() for t in (q, k, v, table))
+    w = torch.ones(32)
+    x = [be.to(t.contiguous()).requires_grad_() for t in (q, k, v, table, w, w)]
+    out = A.rel_attention(*x[:4], _plan_on(be, plan))
+    g, = torch.autograd.grad(out.square().sum(), x[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum() + x[0].sum(), x[0])
+    qn, kn = A.qk_norm_rope(x[0], x[1], x[4], x[5])
+    g, = torch.autograd.grad(qn.square().sum() + kn.sum(), x[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(g.sum() + x[0].sum(), x[0])
