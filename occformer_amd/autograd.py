@@ -10,7 +10,6 @@ the library.  Parameters enter as Function inputs so autograd accumulates into t
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import fused, noise
 from .ops import get_ops
@@ -596,6 +595,36 @@ class MaskedAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
+class _FirstOrder(torch.autograd.Function):
+    """hands the first ``count`` tensors on; their derivative with respect to any of the others does not exist here"""
+
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what}: the gradients come from kernels of their own and are not differentiable again")
+
+
+def _first_order_only(backward):
+    """A backward whose gradients, asked for with create_graph, raise when they are differentiated.  (torch's
+    ``once_differentiable`` leaves its error off every path to the inputs: ``torch.autograd.grad`` for given inputs does not
+    meet it and drops the terms.)"""
+    def wrapped(ctx, *grad_outputs):
+        with torch.no_grad():
+            grads = backward(ctx, *grad_outputs)
+        if torch.is_grad_enabled():
+            made = [g for g in grads if g is not None]
+            sources = [t for t in (*grad_outputs, *ctx.saved_tensors) if t is not None and t.requires_grad]
+            if sources:
+                made = iter(_FirstOrder.apply(backward.__qualname__.split(".")[0], len(made), *made, *sources))
+                grads = tuple(None if g is None else next(made) for g in grads)
+        return grads
+    return wrapped
+
+
 class QkNormRope(torch.autograd.Function):
     """``ops.qk_norm_rope`` with its backward; no gradient for the tables and positions"""
 
@@ -606,7 +635,7 @@ class QkNormRope(torch.autograd.Function):
         return get_ops().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, axis_dims, interleaved)
 
     @staticmethod
-    @once_differentiable
+    @_first_order_only
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         dq_out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if dq_out is None else dq_out
@@ -633,7 +662,7 @@ class RelAttention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order_only
     def backward(ctx, dout):
         q, k, v, table, out, lse, q_lens, k_lens, q_start = ctx.saved_tensors
         buckets, scale, causal = ctx.cfg

@@ -177,9 +177,12 @@ def test_second_derivatives_are_refused(be, monkeypatch):
     x = [be.to(t.contiguous()).requires_grad_() for t in (q, k, v, table, w, w)]
     out = A.rel_attention(*x[:4], _plan_on(be, plan))
     g, = torch.autograd.grad(out.square().sum(), x[0], create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
+    with pytest.raises(RuntimeError, match="not differentiable again"):
         torch.autograd.grad(g.sum() + x[0].sum(), x[0])
+    for y in (g.square().sum(), g.sum() + x[0].sum()):
+        with pytest.raises(RuntimeError, match="not differentiable again"):
+            y.backward(retain_graph=True)
     qn, kn = A.qk_norm_rope(x[0], x[1], x[4], x[5])
     g, = torch.autograd.grad(qn.square().sum() + kn.sum(), x[0], create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
+    with pytest.raises(RuntimeError, match="not differentiable again"):
         torch.autograd.grad(g.sum() + x[0].sum(), x[0])
