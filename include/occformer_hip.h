@@ -654,7 +654,7 @@ int occf_qk_norm_rope_bwd(const void* q, const void* k, const void* q_weight, co
  *          buckets (<= 128), R (<= 512), q strides of batch / row / head, k strides, v strides } (elements, 16-byte
  * multiples; rows D or more apart; pointers 16-byte aligned).  table [buckets, Hq], lut [2 R + 1], out [B, Lq, Hq, D] contiguous,
  * lse [B, Hq, Lq] (may be NULL) = base-2 logarithm of a row's sum of exponentials (-inf: no key), what the backward reads.
- * workspace: occf_rel_attn_workspace floats (0: may be NULL; negative: arguments outside the limits). */
+ * workspace: occf_rel_attn_workspace floats on 16 bytes (0: may be NULL; negative: arguments outside the limits). */
 long occf_rel_attn_workspace(const int64_t* geom, int dtype);
 int occf_rel_attn_fwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
                       const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_start, void* out, float* lse,

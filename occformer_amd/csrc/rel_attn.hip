@@ -612,7 +612,7 @@ extern "C" int occf_rel_attn_fwd(const void* q, const void* k, const void* v, co
   RaParams p = ra_params(geom, scale, causal);
   ra_plan(geom, causal, k_lens != nullptr, dtype, few, p.nsplit, p.chunk);
   const long need = occf_rel_attn_workspace(geom, dtype);
-  if (need > 0 && (!workspace || workspace_floats < need)) return OCCF_EINVAL;
+  if (need > 0 && (!workspace || workspace_floats < need || ((uintptr_t)workspace & 15))) return OCCF_EINVAL;
   p.q = q; p.k = k; p.v = v; p.table = table; p.lut = lut;
   p.q_lens = q_lens; p.k_lens = k_lens; p.q_start = q_start;
   p.o = out; p.lse = lse; p.part = few && need > 0 ? workspace : nullptr;

@@ -186,3 +186,22 @@ def test_second_derivatives_are_refused(be, monkeypatch):
     g, = torch.autograd.grad(qn.square().sum() + kn.sum(), x[0], create_graph=True)
     with pytest.raises(RuntimeError, match="not differentiable again"):
         torch.autograd.grad(g.sum() + x[0].sum(), x[0])
+
+
+def test_rel_attention_c_entry_refuses_a_workspace_off_16_bytes(be):
+    """parts of the keys are written and read 16 bytes at a time"""
+    import ctypes
+    B, L, H, D = 1, 1030, 1, 32
+    g = (ctypes.c_int64 * 17)(B, 1, L, H, H, D, 8, 9, *[D * H, D * H, D], *[L * D * H, D * H, D] * 2)
+    lib, n = be.ops.lib, be.ops.lib.occf_rel_attn_workspace
+    need = n(g, 0)
+    assert need > 0
+    q, k, v, table = be.to(_randn((B, 1, H, D), 1), _randn((B, L, H, D), 2), _randn((B, L, H, D), 3), _randn((8, H), 4))
+    lut = _plan_on(be, _attn_inputs(FEW, torch.float32)[4]).lut
+    out, ws = torch.empty_like(q), torch.empty((need + 4,), dtype=torch.float32, device=q.device)
+    base = (-ws.data_ptr() % 16) // 4
+    for off in (1, 2, 3):
+        ptr = [q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), lut.data_ptr(), None, None, None, out.data_ptr(), None,
+               ws[(base + off) % 4:].data_ptr()]
+        assert (ptr[-1] % 16) != 0
+        assert lib.occf_rel_attn_fwd(*ptr, need, g, 1.0, 0, 0, ctypes.c_void_p(0)) < 0
