@@ -662,7 +662,8 @@ int occf_rel_attn_fwd(const void* q, const void* k, const void* v, const void* t
                       void* stream);
 
 /* Its backward: out / lse as the forward left them, dout [B, Lq, Hq, D]; dq [B, Lq, Hq, D], dk / dv [B, Lk, Hk, D] (rows that
- * do not count are zeros), dtable [buckets, Hq].  Every sum in a fixed order: two runs give the same bits. */
+ * do not count are zeros), dtable [buckets, Hq].  Every sum in a fixed order: two runs give the same bits.  Hq D < 2^22;
+ * workspace: occf_rel_attn_bwd_workspace floats on 16 bytes (negative: arguments outside the limits). */
 long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype);
 int occf_rel_attn_bwd(const void* q, const void* k, const void* v, const void* table, const int32_t* lut,
                       const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_start, const void* out,

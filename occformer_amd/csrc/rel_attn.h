@@ -219,7 +219,7 @@ template <int DP> struct RaRow {
 typedef uint32_t ra_u2 __attribute__((ext_vector_type(2)));
 
 // bounded loads (no branch a load: under branches every load is waited for where the paths meet).  The resource starts at the
-// tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows span less than 2 GiB (ra_check)
+// tile's first row, so that 32-bit offsets reach it wherever it lies; a tile's rows span less than 2 GiB (ra_check, ra_bwd_check)
 #ifdef OCCF_EMU
 static inline RaU4 ra_buf16(occf_bbuf b, uint32_t off) {
   const occf_u32x4 v = occf_bbuf_load_b128(b, off);

@@ -630,8 +630,15 @@ static int ra_bwd(const RaBwd& g, void* stream) {
   else return g.a.Lq <= 512 && g.a.Lk <= 512 ? ra_bwd_run<T, DP, 2>(g, stream) : ra_bwd_run<T, DP, 1>(g, stream);
 }
 
+// rows of dO lie Hq D elements apart: 64 of them within 2 GiB, as ra_check has it for q, k and v (heads of q that are one head
+// repeated may be many and lie close)
+static int ra_bwd_check(const int64_t* g, int dtype) {
+  const int bad = ra_check(g, dtype);
+  return bad ? bad : g[3] * g[5] >= (1L << 22) ? OCCF_ESHAPE : 0;
+}
+
 extern "C" long occf_rel_attn_bwd_workspace(const int64_t* geom, int causal, int dtype) {
-  if (ra_check(geom, dtype)) return -1;
+  if (ra_bwd_check(geom, dtype)) return -1;
   int qs, ks;
   ra_bwd_plan(geom, causal, dtype, qs, ks);
   const RaBwdSizes s = ra_bwd_sizes(geom, qs, ks);
@@ -643,7 +650,7 @@ extern "C" int occf_rel_attn_bwd(const void* q, const void* k, const void* v, co
                                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* dtable,
                                  float* workspace, long workspace_floats, const int64_t* geom, float scale, int causal,
                                  int dtype, void* stream) {
-  const int bad = ra_check(geom, dtype);
+  const int bad = ra_bwd_check(geom, dtype);
   if (bad) return bad;
   if (!q || !k || !v || !table || !lut || !out || !lse || !dout || !dq || !dk || !dv || !dtable || !workspace || !(scale > 0.f))
     return OCCF_EINVAL;

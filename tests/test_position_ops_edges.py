@@ -205,3 +205,16 @@ def test_rel_attention_c_entry_refuses_a_workspace_off_16_bytes(be):
                ws[(base + off) % 4:].data_ptr()]
         assert (ptr[-1] % 16) != 0
         assert lib.occf_rel_attn_fwd(*ptr, need, g, 1.0, 0, 0, ctypes.c_void_p(0)) < 0
+
+
+def test_rel_attention_backward_refuses_gradient_rows_too_far_apart(be):
+    """rows of the gradient of the output lie Hq D elements apart, whatever the strides of q say (one head repeated)"""
+    import ctypes
+    for Hq, D, ok in ((1 << 19, 8, False), ((1 << 19) - 1, 8, True), (1 << 16, 64, False)):
+        g = (ctypes.c_int64 * 17)(1, 2, 2, Hq, 1, D, 8, 9, *[2 * D, D, 0], *[2 * D, D, 0] * 2)
+        for dtype in (0, 1):
+            assert (be.ops.lib.occf_rel_attn_bwd_workspace(g, 0, dtype) > 0) == ok
+            n = ctypes.c_void_p(16)
+            if not ok:
+                assert be.ops.lib.occf_rel_attn_bwd(*[n] * 16, 1 << 40, g, 1.0, 0, dtype, ctypes.c_void_p(0)) < 0
+            assert be.ops.lib.occf_rel_attn_workspace(g, dtype) >= 0       # the forward has no such rows
