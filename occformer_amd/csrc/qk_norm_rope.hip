@@ -219,9 +219,12 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QnParams p) {
         second = o >= tail;
         pr = p.half + (second ? o - tail : o);
       }
-      float sum = 0.f;
-      for (int k = 0; k < rpb; ++k) sum += acc[((k * lpr) * V + pr) * 2 + second];
-      p.part[(long)blockIdx.x * p.D + t] = sum;
+      // four sums side by side, then in pairs: a quarter of the roundings at the size of the whole
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < rpb; k += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += acc[(((k + e) * lpr) * V + pr) * 2 + second];
+      p.part[(long)blockIdx.x * p.D + t] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
   }
 }
@@ -243,9 +246,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_dw_kernel(const float* __res
   acc[r][threadIdx.x & 7] = sum;
   __syncthreads();
   if (r == 0 && c < D) {
-    float t = 0.f;
-    for (int i = 0; i < 32; ++i) t += acc[i][threadIdx.x & 7];
-    qn_put((which ? dwk : dwq)[c], t);
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 32; i += 4)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] += acc[i + e][threadIdx.x & 7];
+    qn_put((which ? dwk : dwq)[c], (t[0] + t[1]) + (t[2] + t[3]));
   }
 }
 

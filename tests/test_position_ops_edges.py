@@ -218,3 +218,23 @@ def test_rel_attention_backward_refuses_gradient_rows_too_far_apart(be):
             if not ok:
                 assert be.ops.lib.occf_rel_attn_bwd(*[n] * 16, 1 << 40, g, 1.0, 0, dtype, ctypes.c_void_p(0)) < 0
             assert be.ops.lib.occf_rel_attn_workspace(g, dtype) >= 0       # the forward has no such rows
+
+
+def test_qk_norm_rope_weight_gradient_sums(be):
+    """the weights' gradient over N = 10 000 rows, by its roundings (each u sqrt(1/3) 0.74 of its value in the mean square, for values
+    spread over a binade).  Independent terms of size s leave s sqrt(k) behind k of them, so that a chain of n equal parts rounds as
+    often as (n + 1) / 2 additions of the whole.  16 of a workgroup's 64 rows in a row: 8.5, two steps of pairs 2; 5 of 157
+    workgroups 3, 8 of 32 such 4.5, pairs 2: together 20, and 0.5 u^2 of a term's own make a root of 0.5 + 20 * 0.18: 2.0 u s sqrt(N).
+    (64 rows and 32 sums one after the other: 52 -> 3.1.)  Bound: half-way, over 6 seeds of two weights of 32 columns."""
+    B, L, H, D = 1, 2500, 4, 32
+    total = 0.0
+    for seed in range(6):
+        x, dz = _randn((2, B, L, H, D), 70 + seed, 2.0), _randn((2, B, L, H, D), 90 + seed)
+        w = torch.ones(D)
+        dw = be.ops.qk_norm_rope_backward(*be.to(x[0], x[1], w, w, dz[0], dz[1]))[2:]
+        for i in (0, 1):
+            xd = x[i].double()
+            terms = dz[i].double() * xd * (xd.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+            err = (dw[i].cpu().double() - terms.sum((0, 1, 2))) / (U * terms.square().sum((0, 1, 2)).sqrt())
+            total += float(err.square().mean())
+    assert (total / 12) ** 0.5 <= 2.6
