@@ -1305,7 +1305,8 @@ class HipOps:
             for name, x, g in (("dq_out", q, dq_out), ("dk_out", k, dk_out)):
                 if (x is None) != (g is None) or (x is not None and (g.shape != x.shape or g.dtype != q.dtype)):
                     raise OccfError(f"{what}: {name} must have the shape and type of its output")
-            dq_out, dk_out = (None if g is None else self._aligned(g.contiguous()) for g in (dq_out, dk_out))
+            on16 = lambda g: g if g.data_ptr() % 16 == 0 else g.clone()      # (the kernel picks its loads by the rows' length)
+            dq_out, dk_out = (None if g is None else on16(g.contiguous()) for g in (dq_out, dk_out))
         strides = q.stride()[:3] + ((0, 0, 0) if k is None else k.stride()[:3])
         geom = (ctypes.c_int64 * 17)(B, L, Hq, 0 if k is None else k.shape[2], D, rot, rows, axes, c1, c2, per_b, *strides)
         taken = (q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out)

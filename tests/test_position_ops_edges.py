@@ -238,3 +238,20 @@ def test_qk_norm_rope_weight_gradient_sums(be):
             err = (dw[i].cpu().double() - terms.sum((0, 1, 2))) / (U * terms.square().sum((0, 1, 2)).sqrt())
             total += float(err.square().mean())
     assert (total / 12) ** 0.5 <= 2.6
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 6), (torch.bfloat16, 10), (torch.bfloat16, 24), (torch.float32, 128)])
+def test_qk_norm_rope_takes_gradients_as_they_are(be, dtype, D):
+    """contiguous gradients on 16 bytes go to the kernel whatever their rows' length, and their layout is checked once"""
+    q, w = be.to(_randn((2, 5, 3, D), 1).to(dtype), torch.ones(D, dtype=dtype))
+    dz = be.to(_randn((2, 5, 3, D), 2).to(dtype))
+    args = (q, None, w, None, None, None, None, dz, None)
+    plan, taken = be.ops._check_norm(*args, None, False, "qk_norm_rope_backward")
+    assert taken[7] is dz
+    before = be.ops.qk_norm_rope_backward(q, None, w, None, dz, None)
+    assert be.ops._plan(be.ops._check_norm, args, None, False, "qk_norm_rope_backward")[0] is \
+        be.ops._plan(be.ops._check_norm, args, None, False, "qk_norm_rope_backward")[0]
+    off = torch.empty((dz.numel() + 1,), dtype=dtype, device=dz.device)[1:].view(dz.shape)
+    off.copy_(dz)                                                        # off 16 bytes: copied, not refused
+    for a, b in zip(before, be.ops.qk_norm_rope_backward(q, None, w, None, off, None)):
+        assert a is None or torch.equal(a, b)
