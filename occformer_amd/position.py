@@ -52,4 +52,4 @@ class RelativeBuckets:
 
     def bucket(self, distance):
         """bucket of every entry of an integer tensor of distances (key - query)"""
-        return self.lut[distance.clamp(-self.radius, self.radius).long() + self.radius]
+        return self.lut[distance.long().clamp(-self.radius, self.radius) + self.radius]

@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from occformer_amd.position import RelativeBuckets
 from tests.test_position_ops import BF, NAN, U, _attn_inputs, _attn_ref, _half, _plan_on, _randn, _within
 
 # few queries; enough heads that the kernel for many queries takes the call (B, Lq, Lk, Hq, Hk, D, causal, buckets, radius, both
@@ -255,3 +256,15 @@ def test_qk_norm_rope_takes_gradients_as_they_are(be, dtype, D):
     off.copy_(dz)                                                        # off 16 bytes: copied, not refused
     for a, b in zip(before, be.ops.qk_norm_rope_backward(q, None, w, None, off, None)):
         assert a is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16, torch.int32, torch.int64])
+def test_relative_buckets_of_any_integer_type(dtype):
+    """a radius that the distances' type cannot hold"""
+    plan = RelativeBuckets(32, 400, True, device="cpu")
+    top = min(torch.iinfo(dtype).max, 1000)
+    d = torch.tensor([0, 1, 5, 100, top], dtype=dtype)
+    assert torch.equal(plan.bucket(d), plan.bucket(d.long()))
+    assert [int(plan.bucket(d)[i]) for i in range(5)] == [int(plan.lut[400 + min(int(x), 400)]) for x in d]
+    if dtype != torch.uint8:
+        assert torch.equal(plan.bucket(-d), plan.bucket(-d.long()))
