@@ -266,6 +266,7 @@ static int qn_setup(QnParams& p, const void* q, const void* k, const void* qw, c
   if (rot && (!cos || !sin || P <= 0 || axes < 1 || axes > 3 || (axes > 1 && !pos))) return OCCF_EINVAL;
   if (rot && axes > 1 && (g[8] < 1 || g[9] < g[8] || (axes == 2 && g[9] < rot / 2))) return OCCF_EINVAL;   // no column of a third axis
   if (B * L * (Hq > Hk ? Hq : Hk) >= 2147483647L) return OCCF_ESHAPE;
+  if (P > 2147483647L || g[8] > D || g[9] > D) return OCCF_ESHAPE;
   const int esize = dtype == 0 ? 4 : 2, pairs = (int)D / 2, half = (int)rot / 2;
   // the widest vectors that the columns, the strides and the addresses allow: 16 bytes a load, else half that, else single pairs
   uintptr_t align = (uintptr_t)q | (uintptr_t)k | (uintptr_t)qw | (uintptr_t)kw;

@@ -268,3 +268,15 @@ def test_relative_buckets_of_any_integer_type(dtype):
     assert [int(plan.bucket(d)[i]) for i in range(5)] == [int(plan.lut[400 + min(int(x), 400)]) for x in d]
     if dtype != torch.uint8:
         assert torch.equal(plan.bucket(-d), plan.bucket(-d.long()))
+
+
+def test_qk_norm_rope_c_entry_refuses_sizes_beyond_32_bits(be):
+    """table rows and axis cuts are 32-bit numbers in the kernel"""
+    import ctypes
+    q, w = be.to(_randn((1, 4, 2, 8), 1), torch.ones(8))
+    cos, sin = be.to(torch.ones(8, 4), torch.zeros(8, 4))
+    pos, out = be.to(torch.zeros((4, 2), dtype=torch.int32)), torch.empty_like(q)
+    for rows, cuts in ((1 << 31, (2, 4)), ((1 << 32) + 8, (2, 4)), (8, (2, (1 << 32) + 2)), (8, ((1 << 32) + 1, (1 << 32) + 4))):
+        g = (ctypes.c_int64 * 17)(1, 4, 2, 0, 8, 8, rows, 2, *cuts, 0, 64, 16, 8, 0, 0, 0)
+        ptr = [t if t is None else t.data_ptr() for t in (q, None, w, None, cos, sin, pos, out, None)]
+        assert be.ops.lib.occf_qk_norm_rope_fwd(*ptr, g, 1e-6, 0, 0, ctypes.c_void_p(0)) < 0
