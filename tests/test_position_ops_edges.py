@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from occformer_amd.position import RelativeBuckets
-from tests.test_position_ops import BF, NAN, U, _attn_inputs, _attn_ref, _half, _plan_on, _randn, _within
+from tests.test_position_ops import NAN, U, _attn_inputs, _attn_ref, _check_attention, _plan_on, _randn, _within
 
 # few queries; enough heads that the kernel for many queries takes the call (B, Lq, Lk, Hq, Hk, D, causal, buckets, radius, both
 # sides, rows)
@@ -280,3 +280,17 @@ def test_qk_norm_rope_c_entry_refuses_sizes_beyond_32_bits(be):
         g = (ctypes.c_int64 * 17)(1, 4, 2, 0, 8, 8, rows, 2, *cuts, 0, 64, 16, 8, 0, 0, 0)
         ptr = [t if t is None else t.data_ptr() for t in (q, None, w, None, cos, sin, pos, out, None)]
         assert be.ops.lib.occf_qk_norm_rope_fwd(*ptr, g, 1e-6, 0, 0, ctypes.c_void_p(0)) < 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1, 9, 640, 2, 1, 32, True, 128, 512, False, [(9, 640, 631)]),
+                                  (1, 40, 70, 2, 2, 128, False, 128, 512, True, [(40, 70, -300)]),
+                                  (1, 33, 40, 1, 1, 64, False, 128, 100, True, None)])
+def test_rel_attention_most_buckets_and_widest_radius(be, case, dtype):
+    _check_attention(be, case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rel_attention_more_sequences_than_parts_are_counted_for(be, dtype):
+    n = [(7 * b) % 34 for b in range(520)]
+    _check_attention(be, (520, 1, 33, 2, 1, 8, True, 8, 40, False, [(1, m, m - 1) for m in n]), dtype, backward=False)
