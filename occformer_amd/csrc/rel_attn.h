@@ -392,6 +392,12 @@ __device__ __forceinline__ f32x4 ra_mm16(const RaFrag<NT>& a, const RaFrag<NT>& 
   return ra_mfma16(a.p[0], b.p[0], c);
 }
 
+// bf16 rows times values in two pieces
+__device__ __forceinline__ f32x4 ra_mm16(const RaFrag<1>& a, const RaFrag<2>& b, f32x4 c) {
+  c = ra_mfma16(a.p[0], b.p[1], c);
+  return ra_mfma16(a.p[0], b.p[0], c);
+}
+
 // a table entry in the base-2 domain; entries at or under -1e30 take their bucket out
 __device__ __forceinline__ float ra_bias(float x) { return x <= -1e30f ? -INFINITY : x * RA_LOG2E; }
 

@@ -20,7 +20,8 @@
 // workgroups a compute unit: one's exponentials run beside the other's products.  2 x 4096 causal rows, 16 heads of 64: 104 us,
 // 660 TFLOP/s of the two products; 8192 rows, 16 heads of 128: 303 us, 906 TFLOP/s.  Bound by what is left of the softmax beside
 // the products.  Tried at these two (at 104 and 330 us): a second image and one barrier a tile, 115 and 436 (the offsets cost a
-// wave a SIMD); tiles of 32 keys, 165 and 434; Q K^T of the next tile in one block with this one's exponentials, 144 and 567.
+// wave a SIMD); tiles of 32 keys, 165 and 434; probabilities in two bf16 pieces, 134 and 427 against 312, so that bf16 ones go into
+// their product (not into their sum) rounded to bf16: the output is off by 2.1e-3 where its own rounding is 1.7e-3; Q K^T of the next tile in one block with this one's exponentials, 144 and 567.
 template <class T, int DP, int KT>
 struct RaFwd {
   static constexpr int tile = 2 * RaType<T>::NT * RaRow<DP>::bytes(KT);                  // K and V
@@ -226,6 +227,8 @@ __device__ __forceinline__ bool ra_unit(const RaParams& p, int unit, int seq, in
 // keys, 8 key heads of 128: 46 us a launch among others on the same keys, part of them still cached, 67 us a call (with the join)
 // on others; 4 x 2500 fp32 queries and keys, 4 heads of 32: 61 us, bound by the six products a score and their operands'
 // splitting.
+// bf16: probabilities go into their product as two bf16 pieces (2^-16), which the stream hides: 67.2 us for the single queries
+// above either way, 86.4 instead of 85.9 for forward and backward of 3 x 777 rows, 12 heads of 64.
 // part != NULL: unnormalised sums, maxima and sums of exponentials of a split.
 template <class T, int DP, int RW>
 struct RaFew {
@@ -332,7 +335,8 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
   Acc acc[DT];
   float m, mref, l;
   const auto walk = [&](auto any) {
-    constexpr bool ANY = decltype(any)::value;           // (ra_split2_any)
+    constexpr bool ANY = decltype(any)::value;           // with infinities (ra_split2_any)
+    constexpr int NP = NT == 3 ? 3 : ANY ? 1 : 2;        // pieces of a probability
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -404,28 +408,27 @@ __global__ void __launch_bounds__((RaFew<T, DP, RW>::NW * 64), RaType<T>::NT == 
       l += sum;
 #pragma unroll
       for (int s2 = 0; s2 < NE / 8; ++s2) {
-        const RaFrag<NT> pf = ra_pack8<NT>(pv + s2 * 8);
+        const RaFrag<NP> pf = ra_pack8<NP>(pv + s2 * 8);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          if constexpr (RW == 32) acc[dt] = ra_mm<NT>(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, lane), pf, acc[dt]);
-          else acc[dt] = ra_mm16<NT>(ra_read_trans16<NT, DP>(img_v, dt * 16, lane), pf, acc[dt]);
+          if constexpr (RW == 32) acc[dt] = ra_mm(ra_read_trans<NT, DP, 32>(img_v, dt * 32, s2, lane), pf, acc[dt]);
+          else acc[dt] = ra_mm16(ra_read_trans16<NT, DP>(img_v, dt * 16, lane), pf, acc[dt]);
         }
       }
     }
   };
   walk(std::false_type());
-  if constexpr (NT == 3) {
-    // an infinite, or nearly infinite, key or value leaves NaN behind: this wave's keys once more, split for them (looking for
-    // them ahead of each tile's split costs 4.5 % at 4 x 2500 queries and keys, 4 heads of 32; so it is 1.8 %)
-    bool bad = l != l;
+  // an infinite (fp32: or nearly infinite) key or value leaves NaN behind: inf - inf among its pieces, or inf times a second piece of
+  // zero.  This wave's keys once more, then, split for them, bf16 probabilities in one piece (looking for them ahead of each tile
+  // costs 4.5 % at 4 x 2500 fp32 queries and keys, 4 heads of 32; so it is 1.8 %)
+  bool bad = l != l;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-      for (int r = 0; r < RW * RW / 64; ++r) bad |= acc[dt][r] != acc[dt][r];
-    if (__ballot(bad)) {
-      load(jw);
-      walk(std::true_type());
-    }
+    for (int r = 0; r < RW * RW / 64; ++r) bad |= acc[dt][r] != acc[dt][r];
+  if (__ballot(bad)) {
+    load(jw);
+    walk(std::true_type());
   }
 #pragma unroll
   for (int mm = RW; mm < 64; mm <<= 1) l += __shfl_xor(l, mm);

@@ -1398,7 +1398,8 @@ class HipOps:
         j <= p_i; other rows, and rows that see no key, are zeros.  A table entry at or below -1e30 takes its bucket out.
         One query of a sequence that grows: q_start = k_lens - 1.  fp32 or bf16 -> [B, Lq, Hq, D]; with ``return_lse`` also the
         rows' base-2 logarithms of the sum of exponentials, fp32 [B, Hq, Lq], for ``rel_attention_backward``.
-        bf16: probabilities are rounded to bf16 before the product with v, not before their sum."""
+        bf16: probabilities go into the product with v as two bf16 pieces (2^-16), from as many queries as fill the card on
+        rounded to bf16, never into their sum."""
         causal = bool(causal)
         (_, dt, geom, scale, need), (q, k, v, _, _, table, lut, q_lens, k_lens, q_start, _) = self._plan(
             self._check_rel_attention, (q, k, v, None, None, table, buckets.lut, q_lens, k_lens, q_start, None),
