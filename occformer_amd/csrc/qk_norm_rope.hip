@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QnParams p) {
   const int lpr = p.lpr, rpb = 256 / lpr;                 // lanes a row, rows a workgroup and step
   const int lane = threadIdx.x % lpr, slot = threadIdx.x / lpr;
   const int pc = lane * V, pairs = p.D / 2;
-  const bool on = pc < pairs;
+  const bool on = pc < pairs, turned = pc < p.half;       // (a load's pairs are turned or not together)
   const int tail = pairs - p.half;                        // pairs of the columns that are not turned
   const int ca = INTER ? 2 * pc : (pc < p.half ? pc : 2 * p.half + pc - p.half);
   const int cb = INTER ? 0 : (pc < p.half ? pc + p.half : ca + tail);
@@ -161,8 +161,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QnParams p) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const float ya = a[e] * rs * wa[e], yb = b[e] * rs * wb[e];
-          a[e] = fmaf(ya, c[e], -(yb * sn[e]));
-          b[e] = fmaf(yb, c[e], ya * sn[e]);
+          a[e] = turned ? fmaf(ya, c[e], -(yb * sn[e])) : ya;       // (0 times a partner's NaN is no zero)
+          b[e] = turned ? fmaf(yb, c[e], ya * sn[e]) : yb;
         }
         qn_store<T, V, INTER>((T*)s.out + row * p.D, ca, cb, a, b);
       }
@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QnParams p) {
         qn_load<T, V, INTER>((const T*)s.dz + row * p.D, ca, cb, ga, gb);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float ya = fmaf(ga[e], c[e], gb[e] * sn[e]), yb = fmaf(gb[e], c[e], -(ga[e] * sn[e]));
+          const float ya = turned ? fmaf(ga[e], c[e], gb[e] * sn[e]) : ga[e];
+          const float yb = turned ? fmaf(gb[e], c[e], -(ga[e] * sn[e])) : gb[e];
           a[e] *= rs;
           b[e] *= rs;
           da[e] = fmaf(ya, a[e], da[e]);

@@ -307,3 +307,18 @@ def test_rel_attention_few_queries_round_once(be, case):
     want = _attn_ref(q, k, v, table, plan, case[6], case[5] ** -0.5, *lens, None, torch.bfloat16)["out"][0]
     out = be.ops.rel_attention(*be.to(q, k, v, table), _plan_on(be, plan), causal=case[6], k_lens=be.to(lens[1]), q_start=be.to(lens[2]))
     assert float((out.cpu().double() - want).norm()) <= 1.1 * float((want.bfloat16().double() - want).norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inter", [False, True])
+def test_qk_norm_rope_infinity_stays_in_its_column(be, inter, dtype):
+    """a row with an infinity: its root mean square is infinite, so every finite column comes out as zero and the infinite one as NaN,
+    which the rotation takes to its partner, but the columns that are not turned have none"""
+    D, half = 32, 4
+    q, w = _randn((1, 3, 1, D), 1).to(dtype), torch.ones(D, dtype=dtype)
+    q[0, 1, 0, 20] = math.inf
+    for rot in (None, half):
+        cos, sin = (None, None) if rot is None else be.to(torch.full((4, half), 0.6), torch.full((4, half), 0.8))
+        out = be.ops.qk_norm_rope(be.to(q), None, be.to(w), None, cos, sin, interleaved=inter)[0].cpu()
+        assert bool(out[0, 1, 0, 20].isnan()) and int((out[0, 1, 0] == 0).sum()) == D - 1
+        assert bool(out[0, 0].isfinite().all()) and bool(out[0, 2].isfinite().all())
