@@ -10,8 +10,8 @@
 // One pass, bound by the memory stream: a row is VEC pairs a lane, its D / 2 / VEC lanes (rounded up to a power of two) sum
 // the squares by shuffles, so that a row is read once and written once; the angles' cosines and sines come from a table made
 // in 64 bits (a far position's angle loses digits in 32) whose row is shared by the heads of a token.
-// Forward, 2 x 8192 tokens of 32 + 8 bf16 heads of 128: 68.5 us, 5.0 TB/s.  Backward, 4 x 4095 tokens of 16 + 4 bf16 heads of
-// 64: 25 us, 5.0 TB/s, and 4 us for the weights' sums of at most 512 workgroups a side, in their order.
+// Forward, 2 x 8192 tokens of 32 + 8 bf16 heads of 128: 68.5 us, 5.0 TB/s.  4 x 4095 tokens of 16 + 4 bf16 heads of 64:
+// 21 us, backward 28.6 us, 4.4 TB/s, and 3.9 us for the weights' sums of at most 512 workgroups a side, in a fixed order.
 #include "occf_common.h"
 #include "../../include/occformer_hip.h"
 

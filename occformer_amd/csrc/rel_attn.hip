@@ -17,9 +17,11 @@
 // ---------------------------------------------------------------------------------------------------------------------
 // Many queries: a workgroup owns 128 queries of one head, a wave 32 of them (a lane one query: its running maximum and sum
 // are registers), and walks the keys in tiles of KT through LDS; the next tile's rows travel from memory meanwhile.  Two
-// workgroups a compute unit: one's exponentials run beside the other's products.  2 x 4096 causal rows, 16 heads of 64: 104 us,
-// 660 TFLOP/s of the two products; 8192 rows, 16 heads of 128: 303 us, 906 TFLOP/s.  Bound by what is left of the softmax beside
-// the products.  Tried at these two (at 104 and 330 us): a second image and one barrier a tile, 115 and 436 (the offsets cost a
+// workgroups a compute unit: one's exponentials run beside the other's products.  2 x 4096 causal rows, 16 heads of 64: 95 us,
+// 720 TFLOP/s of the two products; 8192 rows, 16 heads of 128: 308 us, 890 TFLOP/s.  Of that time the matrix pipes are busy 30 and
+// 39 %, vector instructions 52 and 35, the LDS 32 and 40: bound by a wave's chain from scores over exponentials to the second product,
+// which two waves a SIMD fill in part.  Tried at these two (at 104 and 330 us; comparisons are of short runs, in which the card has
+// not reached its clock): a second image and one barrier a tile, 115 and 436 (the offsets cost a
 // wave a SIMD); tiles of 32 keys, 165 and 434; probabilities in two bf16 pieces, 134 and 427 against 312, so that bf16 ones go into
 // their product (not into their sum) rounded to bf16: the output is off by 2.1e-3 where its own rounding is 1.7e-3; Q K^T of the next tile in one block with this one's exponentials, 144 and 567.
 template <class T, int DP, int KT>
@@ -224,9 +226,8 @@ __device__ __forceinline__ bool ra_unit(const RaParams& p, int unit, int seq, in
 // waits for another before the join at the end.  (Keys through LDS, in whole rows of the cache line, took 99 instead of 67 us for
 // 4 x 2500 fp32 queries and as long for single ones.)  Bound by the stream of keys and values: 16 rows take half the
 // accumulators, products and exponentials of 32, which leaves room for a second tile in flight.  16 sequences of up to 8192 bf16
-// keys, 8 key heads of 128: 46 us a launch among others on the same keys, part of them still cached, 67 us a call (with the join)
-// on others; 4 x 2500 fp32 queries and keys, 4 heads of 32: 61 us, bound by the six products a score and their operands'
-// splitting.
+// keys, 8 key heads of 128: 59 us, 4.8 TB/s, and 8.5 for the join; 4 x 2500 fp32 queries and keys, 4 heads of 32: 58 us, vector
+// instructions busy 55 % of it (a score's bias, exponential and pieces, the keys' splitting), the matrix pipes 23 %.
 // bf16: probabilities go into their product as two bf16 pieces (2^-16), which the stream hides: 67.2 us for the single queries
 // above either way, 86.4 instead of 85.9 for forward and backward of 3 x 777 rows, 12 heads of 64.
 // part != NULL: unnormalised sums, maxima and sums of exponentials of a split.

@@ -16,9 +16,10 @@
 // the dS so formed ARE that error (P sums to one), so the first kernel adds them to the delta that the second one reads, and
 // takes (row sum) x (P K) off its own dQ: one product more, bf16 only; an fp32 O leaves nothing to correct in dQ.
 //
-// 2 x 4096 causal bf16 rows, 16 / 4 heads of 64: 152 and 235 us, 900 and 585 TFLOP/s of four products each.  The first kernel is
-// bound by the products and the exponentials beside them, the second by the LDS: its operands come as rows and as columns, and
-// the diagonals' sums go through it.  2 x 1000 fp32 rows, 8 heads of 24: 31 and 46 us, short walks of 256 and 512 workgroups.
+// 2 x 4096 causal bf16 rows, 16 / 4 heads of 64: 141 and 198 us, 970 and 690 TFLOP/s of four products each.  Matrix pipes, vector
+// instructions and LDS are busy 42, 43 and 27 % of the first, 26, 32 and 33 % of the second, whose operands come as rows and as columns
+// and whose diagonals' sums go through the LDS between barriers.  2 x 1000 fp32 rows, 8 heads of 24: 29 and 39 us, short walks of
+// 256 and 512 workgroups.  (Comparisons below are of short runs, in which the card has not reached its clock: up to a fifth more.)
 //
 // Both walks are cut into `splits` where whole ones would not fill the card; rel_attn_finish_kernel adds the parts up in order.
 #include "rel_attn.h"

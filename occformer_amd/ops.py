@@ -1395,7 +1395,8 @@ class HipOps:
         """softmax(scale q k^T + table[bucket(j - p_i)]) v with p_i = q_start[b] + i: q [B, Lq, Hq, D], k and v [B, Lk, Hk, D]
         (any strides with contiguous columns; query head h reads key head h // (Hq / Hk)), table [buckets, Hq] the learned bias,
         ``buckets`` a ``position.RelativeBuckets``.  Rows i < q_lens[b] see the keys j < k_lens[b], with ``causal`` those at
-        j <= p_i; other rows, and rows that see no key, are zeros.  A table entry at or below -1e30 takes its bucket out.
+        j <= p_i; other rows, and rows that see no key, are zeros.  (A NaN or infinity in v at a key that counts may reach rows of its
+        tile that do not see it: the product holds a zero for the pair.)  A table entry at or below -1e30 takes its bucket out.
         One query of a sequence that grows: q_start = k_lens - 1.  fp32 or bf16 -> [B, Lq, Hq, D]; with ``return_lse`` also the
         rows' base-2 logarithms of the sum of exponentials, fp32 [B, Hq, Lq], for ``rel_attention_backward``.
         bf16: probabilities go into the product with v as two bf16 pieces (2^-16), from as many queries as fill the card on
