@@ -596,12 +596,12 @@ class MaskedAttention(torch.autograd.Function):
 
 
 class _FirstOrder(torch.autograd.Function):
-    """hands the first ``count`` tensors on; their derivative with respect to any of the others does not exist here"""
+    """copies of the first ``count`` tensors, whose derivative with respect to any of the others does not exist here"""
 
     @staticmethod
     def forward(ctx, what, count, *tensors):
         ctx.what = what
-        return tuple(t.view_as(t) for t in tensors[:count])
+        return tuple(t.clone() for t in tensors[:count])
 
     @staticmethod
     def backward(ctx, *grads):

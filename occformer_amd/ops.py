@@ -1415,8 +1415,8 @@ class HipOps:
     def rel_attention_backward(self, q, k, v, table, buckets, out, lse, dout, scale=None, causal=False, q_lens=None,
                                k_lens=None, q_start=None):
         """-> (dq, dk, dv, dtable) for ``rel_attention``'s out, lse and the gradient dout of out; rows that do not count get
-        zeros.  bf16: P and dS are rounded to bf16 before their products (up to lengths of 512 they go as two bf16 pieces),
-        dtable's sums are not."""
+        zeros.  dout is not looked at behind q_lens; in rows that see no key it has to be finite.  bf16: P and dS are rounded to
+        bf16 before their products (up to lengths of 512 they go as two bf16 pieces), dtable's sums are not."""
         causal = bool(causal)
         (_, dt, geom, scale, need), (q, k, v, out, dout, table, lut, q_lens, k_lens, q_start, lse) = self._plan(
             self._check_rel_attention, (q, k, v, out, dout, table, buckets.lut, q_lens, k_lens, q_start, lse),

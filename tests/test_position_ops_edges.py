@@ -322,3 +322,17 @@ def test_qk_norm_rope_infinity_stays_in_its_column(be, inter, dtype):
         out = be.ops.qk_norm_rope(be.to(q), None, be.to(w), None, cos, sin, interleaved=inter)[0].cpu()
         assert bool(out[0, 1, 0, 20].isnan()) and int((out[0, 1, 0] == 0).sum()) == D - 1
         assert bool(out[0, 0].isfinite().all()) and bool(out[0, 2].isfinite().all())
+
+
+def test_gradients_kept_for_a_graph_can_be_changed_in_place(be, monkeypatch):
+    """gradients asked for with create_graph are tensors of their own: scaling one in place is nobody's business"""
+    from occformer_amd import autograd as A
+    monkeypatch.setattr(A, "get_ops", lambda: be.ops)
+    q, k, v, table, plan, _, _ = _attn_inputs(FEW, torch.float32)
+    x = [be.to(t.nan_to_num().contiguous()).requires_grad_() for t in (q, k, v, table)]
+    plain = torch.autograd.grad(A.rel_attention(*x, _plan_on(be, plan)).square().sum(), x)
+    kept = torch.autograd.grad(A.rel_attention(*x, _plan_on(be, plan)).square().sum(), x, create_graph=True)
+    for a, b in zip(plain, kept):
+        assert torch.equal(a, b)
+        b.mul_(2.0)
+        assert torch.equal(2.0 * a, b)
